@@ -34,13 +34,15 @@ BASE_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-r
 _CORE_SOURCES = ("elementwise.cu", "gemm_generic.cu", "attention_generic.cu", "branch_elementwise.cu",
                  "latent_attention.cu", "linear_recurrence.cu", "hyper_elementwise.cu", "sink_attention.cu",
                  "gla_recurrence.cu", "moe.cu", "rotary_attention.cu", "sandwich_elementwise.cu",
-                 "delta_recurrence.cu", "ssd_recurrence.cu", "parallel_block.cu", "layer_norm.cu", "selective_scan.cu")
+                 "delta_recurrence.cu", "ssd_recurrence.cu", "parallel_block.cu", "layer_norm.cu", "selective_scan.cu",
+                 "fork_copy.cu")
 
 # library name -> (sources, defines)
 LIBRARIES: Dict[str, Tuple[Sequence[str], Sequence[str]]] = {
     "core_f32": (_CORE_SOURCES, ("-DTL_DTYPE=0",)),
     "core_bf16": (_CORE_SOURCES, ("-DTL_DTYPE=1",)),
     "sampling": (("sampling.cu",), ()),
+    "beam": (("beam_select.cu",), ()),
     "random_init": (("random_init.cu",), ()),
 }
 

@@ -7,7 +7,7 @@ a CUDA device, a missing library or a launch that the driver rejects raises
 from __future__ import annotations
 
 from ctypes import c_float, c_int, c_longlong, c_void_p
-from typing import Callable, Dict, Optional
+from typing import Callable, Dict, Optional, Sequence
 
 import torch
 
@@ -124,6 +124,31 @@ def _need(t: torch.Tensor, dtype: torch.dtype, what: str, contiguous: bool = Tru
         raise KernelError(f"{what}: tensor must be contiguous")
 
 
+def _here(t: torch.Tensor, what: str) -> None:
+    """Kernels are launched on the current device's current stream: their tensors must lie there."""
+    if not t.is_cuda:
+        raise KernelError(f"{what}: tensor is not on a CUDA device; this package has no CPU path")
+    if t.device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: tensor lies on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _pairs(src: Sequence[int], dst: Sequence[int], limit: int, what: str) -> int:
+    """Checks lists of copies that run in any order; returns how many there are."""
+    n = len(src)
+    if len(dst) != n:
+        raise KernelError(f"{what}s: {n} to read and {len(dst)} to write")
+    if n == 0:
+        return 0
+    if min(src) < 0 or min(dst) < 0 or max(src) >= limit or max(dst) >= limit:
+        raise KernelError(f"{what}s must lie in [0, {limit})")
+    written = set(dst)
+    if len(written) != n:
+        raise KernelError(f"{what}: one is written twice")
+    if not written.isdisjoint(src):
+        raise KernelError(f"{what}: one is both read and written")
+    return n
+
+
 class CoreOps:
     """The kernels of one activation type (float32 or bfloat16)."""
 
@@ -143,7 +168,7 @@ class CoreOps:
                      "tl_clamped_glu", "tl_delta_prep", "tl_conv_state_update", "tl_delta_scan", "tl_silu_rows",
                      "tl_weighted_sum", "tl_close_block", "tl_moe_route_chosen", "tl_qk_whole_norm_cache_write",
                      "tl_ssd_prep", "tl_ssd_walk", "tl_ssd_gate_norm", "tl_layernorm",
-                     "tl_layernorm_add_layernorm", "tl_selective_scan", "tl_conv_silu"):
+                     "tl_layernorm_add_layernorm", "tl_selective_scan", "tl_conv_silu", "tl_copy_slots", "tl_copy_pages"):
             fn = getattr(self.lib, f"{base}_{self.suffix}")
             fn.restype = c_int
             setattr(self, "_" + base, fn)
@@ -1283,6 +1308,82 @@ class CoreOps:
             _ptr(D), _ptr(z), c_int(z.stride(0)), _ptr(state), _ptr(y), _ptr(seq_start), _ptr(seq_slot),
             c_int(T), c_int(seq_slot.numel()), c_int(channels), c_int(N), _stream()), "selective_scan")
 
+    # ---- one sequence going on from another one's cache ------------------------------------------
+    def copy_slots(self, storage: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Row dst[i] of every layer of `storage` ([layers, slots, ...], any type) becomes what row src[i] holds.
+        No row may be written twice or be written and read."""
+        _here(storage, "copy_slots")
+        if storage.dim() < 2 or not storage.is_contiguous():
+            raise KernelError("copy_slots: the storage must be contiguous [layers, slots, ...]")
+        n = _pairs(src, dst, storage.shape[1], "copy_slots: slot")
+        if n == 0 or storage.numel() == 0:
+            return
+        layers, slots = storage.shape[0], storage.shape[1]
+        row = storage.numel() // (layers * slots) * storage.element_size()
+        _check(self._tl_copy_slots(_ptr(storage), c_int(layers), c_int(slots), c_longlong(row), (c_int * n)(*src),
+                                   (c_int * n)(*dst), c_int(n), _stream()), "copy_slots")
+
+    def copy_pages(self, storage: torch.Tensor, pages: int, heads: int, dim: int, vdim: int, src: Sequence[int],
+                   dst: Sequence[int], counts: Sequence[int]) -> None:
+        """The first counts[i] positions of page src[i] into page dst[i], in every layer of `storage` ([layers, n]: per
+        layer the key pages [pages, heads, PAGE, dim], then the value pages [pages, heads, vdim, PAGE]; vdim 0: none).
+        Later positions of dst[i] keep what they hold.  No page may be written twice or be written and read."""
+        _here(storage, "copy_pages")
+        _need(storage, self.act_dtype, "copy_pages storage")
+        if storage.dim() != 2 or min(pages, heads, dim) < 1 or vdim < 0 or \
+                storage.shape[1] < pages * heads * PAGE * (dim + vdim):
+            raise KernelError("copy_pages: the storage must be [layers, key pages and value pages]")
+        n = _pairs(src, dst, pages, "copy_pages: page")
+        if len(counts) != n or (n and not (1 <= min(counts) and max(counts) <= PAGE)):
+            raise KernelError(f"copy_pages: one count of 1 to {PAGE} positions per pair is needed")
+        if n == 0 or storage.shape[0] == 0:
+            return
+        _check(self._tl_copy_pages(_ptr(storage), c_int(storage.shape[0]), c_longlong(storage.shape[1]), c_int(pages),
+                                   c_int(heads), c_int(dim), c_int(vdim), (c_int * n)(*src), (c_int * n)(*dst),
+                                   (c_int * n)(*counts), c_int(n), _stream()), "copy_pages")
+
+
+class BeamOps:
+    """The selection step of a beam search (beam_select.cu)."""
+    MAX_N = 128      # continuations of one sequence
+
+    def __init__(self):
+        lib = build.load_library("beam")
+        P, I, L = c_void_p, c_int, c_longlong
+        self._scratch = lib.tl_beam_scratch_bytes
+        self._scratch.restype, self._scratch.argtypes = L, [I, I, I]
+        self._select = lib.tl_beam_select
+        self._select.restype, self._select.argtypes = I, [P, L, I, I, I, P, I, P, P, P, P, P]
+
+    def select(self, logits: torch.Tensor, scores: torch.Tensor, n: int) -> torch.Tensor:
+        """logits [S * B, V], scores [S, B], both 32-bit.  Returns int32 [3, S, n]: the bits of the values (32-bit
+        floats), the beams, the tokens."""
+        _here(logits, "beam select")
+        _here(scores, "beam select")
+        if logits.dtype != torch.float32 or scores.dtype != torch.float32:
+            raise KernelError("beam select: logits and scores must be 32-bit floats")
+        if logits.dim() != 2 or scores.dim() != 2 or logits.shape[0] != scores.numel():
+            raise KernelError("beam select: logits [sequences * beams, vocabulary] and scores [sequences, beams] are needed, "
+                              f"got {tuple(logits.shape)} and {tuple(scores.shape)}")
+        V = logits.shape[1]
+        if (V > 1 and logits.stride(1) != 1) or not scores.is_contiguous():
+            raise KernelError("beam select: scores and the rows of logits must be contiguous")
+        S, B = scores.shape
+        if S and not 1 <= n <= min(self.MAX_N, B * V):
+            raise KernelError(f"beam select: {n} continuations of {B} beams and {V} tokens (1 to {self.MAX_N} are possible)")
+        ld = logits.stride(0) if S * B > 1 else V
+        if ld < V:
+            raise KernelError("beam select: the rows of logits overlap")
+        out = torch.empty((3, S, n), dtype=torch.int32, device=logits.device)
+        if S == 0:
+            return out
+        # a buffer of this call's own: calls on other streams and recorded graphs share nothing
+        scratch = torch.empty(self._scratch(S * B, V, n), dtype=torch.uint8, device=logits.device)
+        at = out.data_ptr()
+        _check(self._select(logits.data_ptr(), ld, S, B, V, scores.data_ptr(), n, scratch.data_ptr(), at, at + 4 * S * n,
+                            at + 8 * S * n, _stream()), "beam_select")
+        return out
+
 
 class SamplingOps:
     def __init__(self):
@@ -1318,6 +1419,7 @@ class SamplingOps:
 
 _core: dict = {}
 _sampling: list = []
+_beam: list = []
 
 
 def core_ops(act_dtype: torch.dtype) -> CoreOps:
@@ -1330,3 +1432,9 @@ def sampling_ops() -> SamplingOps:
     if not _sampling:
         _sampling.append(SamplingOps())
     return _sampling[0]
+
+
+def beam_ops() -> BeamOps:
+    if not _beam:
+        _beam.append(BeamOps())
+    return _beam[0]
