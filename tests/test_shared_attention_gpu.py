@@ -1,0 +1,232 @@
+"""Decode attention of rows that share leading pages, against a plain implementation in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from torchless_rs_b200.csrc import ops
+from torchless_rs_b200.csrc.attention_shared import SharedAttention
+from torchless_rs_b200.csrc.ops import KernelError
+from torchless_rs_b200.parts.runtime import Workspace
+
+pytestmark = pytest.mark.gpu
+PAGE = 64
+DEV = "cuda"
+
+
+class Setting:
+    """Groups of `beams[g]` rows of length lens[g] whose tables agree in shared[g] columns; pages in random order, numbers that no row
+    sees are NaN."""
+
+    def __init__(self, dtype, nh, nkv, hd, beams, lens, shared, window=None, seed=0, spread=1.5, junk=float("nan"), pages_more=3):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        self.dtype, self.nh, self.nkv, self.hd, self.window = dtype, nh, nkv, hd, window
+        self.beams, self.lens, self.shared = list(beams), list(lens), list(shared)
+        rows = sum(beams)
+        width = max(max(-(-n // PAGE) for n in lens), 1) + 1
+        total = sum(min(c, -(-n // PAGE)) + b * max(0, -(-n // PAGE) - c) for b, n, c in zip(beams, lens, shared)) + pages_more
+        ids = torch.randperm(total, generator=g, device=DEV).tolist()
+        at, table = 0, []
+        for b, n, c in zip(beams, lens, shared):
+            cols = -(-n // PAGE)
+            c = min(c, cols)
+            first = max(0, n - window) // PAGE if window else 0
+            common = ids[at:at + c]
+            at += c
+            for _ in range(b):
+                row = common + ids[at:at + cols - c]
+                at += cols - c
+                table.append([-1] * first + row[first:] + [-1] * (width - cols))
+        self.table = table
+        slots = torch.randperm(rows + 2, generator=g, device=DEV)[:rows]
+        self.page_table = torch.full((rows + 2, width), -1, dtype=torch.int32, device=DEV)
+        self.page_table[slots] = torch.tensor(table, dtype=torch.int32, device=DEV)
+        self.seq_slot = slots.to(torch.int32)
+        self.row_len = [n for b, n in zip(beams, lens) for _ in range(b)]
+        self.seq_len = torch.tensor(self.row_len, dtype=torch.int32, device=DEV)
+        starts = [0]
+        for b in beams:
+            starts.append(starts[-1] + b)
+        self.group_start = torch.tensor(starts, dtype=torch.int32, device=DEV)
+        self.group_pages = torch.tensor(shared, dtype=torch.int32, device=DEV)
+        self.q = (torch.randn((rows, nh * hd), generator=g, device=DEV) * spread).to(dtype)
+        self.k = torch.randn((total, nkv, PAGE, hd), generator=g, device=DEV).to(dtype)
+        self.v = torch.randn((total, nkv, hd, PAGE), generator=g, device=DEV).to(dtype)
+        seen = torch.zeros((total, PAGE), dtype=torch.bool, device=DEV)
+        for row, n in zip(table, self.row_len):
+            for j in range(max(0, n - window) if window else 0, n):
+                seen[row[j // PAGE], j % PAGE] = True
+        self.k[~seen[:, None, :].expand(-1, nkv, -1)] = junk
+        self.v.masked_fill_(~seen[:, None, None, :], junk)
+        self.scale = 1.0 / math.sqrt(hd)
+        self.ws = Workspace(torch.device(DEV))
+
+    def run(self, **change):
+        out = torch.full_like(self.q, 7.0)
+        a = dict(q=self.q, k_pages=self.k, v_pages=self.v, out=out, seq_len=self.seq_len, seq_slot=self.seq_slot, page_table=self.page_table,
+                 group_start=self.group_start, group_pages=self.group_pages, nh=self.nh, nkv=self.nkv, window=self.window, scale=self.scale,
+                 workspace=self.ws, lens=self.lens, shared=self.shared, group_rows=max(self.beams))
+        a.update(change)
+        SharedAttention.get(self.dtype, self.hd).decode(**a)
+        return a["out"]
+
+    def plain(self):
+        """(out, and the weighted sum of |v|), in 64 bits."""
+        rows, G = len(self.table), self.nh // self.nkv
+        out = torch.zeros((rows, self.nh, self.hd), dtype=torch.float64, device=DEV)
+        mass = torch.zeros_like(out)
+        for r, (row, n) in enumerate(zip(self.table, self.row_len)):
+            lo = max(0, n - self.window) if self.window else 0
+            if n == 0:
+                continue
+            places = torch.arange(lo, n, device=DEV)
+            page = torch.tensor(row, device=DEV)[places // PAGE]
+            k, v = self.k[page, :, places % PAGE].double(), self.v[page, :, :, places % PAGE].double()     # [keys, nkv, hd]
+            q = self.q[r].double().view(self.nkv, G, self.hd)
+            p = torch.softmax(torch.einsum("hgd,nhd->hgn", q, k) * self.scale, -1)
+            out[r] = torch.einsum("hgn,nhd->hgd", p, v).reshape(self.nh, self.hd)
+            mass[r] = torch.einsum("hgn,nhd->hgd", p, v.abs()).reshape(self.nh, self.hd)
+        return out.reshape(rows, -1), mass.reshape(rows, -1)
+
+    def check(self, got=None):
+        """bfloat16: a weight is rounded by at most 2^-8 of it, so the sum by 2^-8 of the weighted sum of |v|; the result by 2^-8 of
+        it; 32-bit sums of at most 4096 terms and exponentials are off by less than 2^-12 of that sum together.  32 bits: scores of
+        up to 2^5 off by (head size + 2) 2^-24 of sums of 64-term products (at most 2^7 in all), so weights by 2^-24 * 2^7 * 8 and
+        sums of n terms by 2^-24 n^(1/2) of the sum: 2^-13 of it covers both."""
+        got = self.run() if got is None else got
+        want, mass = self.plain()
+        assert torch.isfinite(got).all()
+        if self.dtype == torch.bfloat16:
+            bound = mass * (2.0 ** -8 + 2.0 ** -12) + want.abs() * 2.0 ** -8 + 1e-30
+        else:
+            bound = mass * 2.0 ** -13 + 1e-30
+        over = ((got.double() - want).abs() / bound).max().item()
+        assert over <= 1.0, over
+
+
+HEADS = [(torch.bfloat16, 8, 2, 64), (torch.bfloat16, 8, 2, 128), (torch.float32, 8, 2, 64), (torch.float32, 8, 2, 128)]
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("lens,shared", [([1], [0]), ([64], [0]), ([65], [1]), ([64], [1]), ([129, 63], [1, 0]), ([200, 1000, 64, 7], [3, 15, 1, 0]),
+                                         ([4000], [60]), ([300, 2500], [0, 30])])
+def test_lengths_and_common_pages(dtype, nh, nkv, hd, lens, shared):
+    Setting(dtype, nh, nkv, hd, [4] * len(lens), lens, shared, seed=sum(lens)).check()
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64), (torch.float32, 128)])
+@pytest.mark.parametrize("nh,nkv", [(1, 1), (3, 1), (4, 2), (5, 5), (12, 2), (14, 2), (16, 1), (33, 3)])
+@pytest.mark.parametrize("beams", [[1], [2, 3], [5, 1, 16]])
+def test_heads_and_beams(dtype, hd, nh, nkv, beams):
+    lens = [333, 130, 700][:len(beams)]
+    Setting(dtype, nh, nkv, hd, beams, lens, [4, 1, 10][:len(beams)], seed=nh + len(beams)).check()
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("window", [1, 63, 64, 65, 200, 1000])
+def test_windows(dtype, nh, nkv, hd, window):
+    Setting(dtype, nh, nkv, hd, [3, 4, 2], [500, 64, 1111], [6, 0, 16], window=window, seed=window).check()
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+def test_a_key_that_stands_out_on_either_side_of_every_border(dtype, nh, nkv, hd):
+    """One key has a score far above the others: the last common one, the first of a row's own, the newest, the first in the window."""
+    for j, window in ((0, None), (127, None), (128, None), (383, None), (399, None), (100, 300), (101, 300)):
+        s = Setting(dtype, nh, nkv, hd, [4], [400], [6], window=window, seed=j)
+        s.k[s.table[0][j // PAGE], :, j % PAGE] = (s.q[0, :hd] * 4).to(dtype) if j >= 400 - (window or 400) else float("nan")
+        s.check()
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+def test_scores_far_apart_and_scale(dtype, nh, nkv, hd):
+    s = Setting(dtype, nh, nkv, hd, [4, 2], [700, 90], [9, 1], spread=0.2, seed=1)
+    s.k.mul_(20.0)                           # scores of a few dozen: most weights are nothing
+    s.check()
+    s.scale = 0.0
+    s.check()
+    s.scale = -0.05
+    s.check()
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+def test_rows_of_length_zero_give_zero(dtype, nh, nkv, hd):
+    s = Setting(dtype, nh, nkv, hd, [2, 3], [0, 77], [0, 1])
+    got = s.run()
+    assert (got[:2] == 0).all()
+    s.check(got)
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+def test_every_way_of_cutting_gives_the_result(dtype, nh, nkv, hd, monkeypatch):
+    from torchless_rs_b200.csrc import attention_shared
+    s = Setting(dtype, nh, nkv, hd, [4, 3], [1000, 333], [12, 3], seed=8)
+    for plan in ((1, 1, 1), (1, 100, 1), (3, 4, 2), (12, 1, 4), (60, 1, 4), (2, 3, 62), (13, 2, 7)):
+        monkeypatch.setattr(attention_shared, "shared_plan", lambda *a, plan=plan: plan)
+        s.check()
+
+
+def test_a_call_that_does_not_say_that_pages_are_shared_gives_the_same():
+    s = Setting(torch.bfloat16, 8, 2, 128, [4, 4], [700, 300], [10, 4], seed=2)
+    s.check(s.run(group_pages=torch.zeros_like(s.group_pages), shared=[0, 0]))
+    want = s.run()
+    # fewer shared columns than the tables have in common
+    s.check(s.run(group_pages=torch.tensor([3, 1], dtype=torch.int32, device=DEV), shared=[3, 1]))
+    # and the same bits again, on another stream, and from two graphs that are replayed in turn
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = s.run()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        out = torch.zeros_like(s.q)
+        with torch.cuda.graph(graph):
+            s.run(out=out)
+        graphs.append((graph, out))
+    for graph, _ in graphs + graphs:
+        graph.replay()
+    torch.cuda.synchronize()
+    for got in [other] + [out for _, out in graphs]:
+        assert torch.equal(got, want)
+    ops.check_kernel_errors()
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.float32, 64)])
+def test_many_groups_and_the_same_result_as_row_by_row(dtype, hd):
+    """Against the decode attention that reads every row's pages for itself."""
+    s = Setting(dtype, 8, 4, hd, [4] * 9, [100 + 173 * i for i in range(9)], [1 + 2 * i for i in range(9)], seed=4, junk=0.0)
+    got = s.run()
+    out = torch.zeros_like(s.q)
+    ops.core_ops(dtype).attn_generic(s.q, s.k, s.v, out, (s.seq_len - 1).contiguous(), torch.arange(36, dtype=torch.int32, device=DEV),
+                                     s.seq_slot, s.page_table, 8, 4, hd, None, s.scale)
+    s.check(got)
+    s.check(out)
+
+
+def test_offsets_beyond_32_bits():
+    """A cache whose pages begin beyond 2^31 numbers."""
+    hd, nkv, pages = 128, 8, 2 ** 31 // (8 * 64 * 128) + 40
+    s = Setting(torch.bfloat16, 16, nkv, hd, [4], [300], [3], seed=5)
+    k = torch.zeros((pages, nkv, PAGE, hd), dtype=torch.bfloat16, device=DEV)
+    v = torch.zeros((pages, nkv, hd, PAGE), dtype=torch.bfloat16, device=DEV)
+    shift = pages - s.k.shape[0]
+    k[shift:], v[shift:] = s.k, s.v
+    far = torch.where(s.page_table >= 0, s.page_table + shift, s.page_table)
+    s.check(s.run(k_pages=k, v_pages=v, page_table=far))
+
+
+@pytest.mark.parametrize("bad", ["type", "cpu", "heads", "q shape", "pages", "lengths", "starts", "too long", "negative", "window", "groups", "table"])
+def test_refusals(bad):
+    s = Setting(torch.bfloat16, 8, 2, 64, [4, 4], [100, 300], [1, 4])
+    change = {"type": dict(q=s.q.float()), "cpu": dict(q=s.q.cpu()), "heads": dict(nh=34), "q shape": dict(q=s.q[:, :256].contiguous()),
+              "pages": dict(v_pages=s.v[1:]), "lengths": dict(seq_len=s.seq_len[:5]), "starts": dict(group_start=s.group_start[:2]),
+              "too long": dict(lens=[100, 10000]), "negative": dict(shared=[-1, 0]), "window": dict(window=0), "groups": dict(group_rows=0),
+              "table": dict(page_table=s.page_table.long())}[bad]
+    with pytest.raises(KernelError):
+        s.run(**change)
+
+
+def test_sizes_without_a_kernel():
+    assert SharedAttention.get(torch.bfloat16, 32) is None and SharedAttention.get(torch.float16, 64) is None
+    assert not SharedAttention.get(torch.bfloat16, 64).takes(34, 2) and SharedAttention.get(torch.float32, 64).takes(64, 2)

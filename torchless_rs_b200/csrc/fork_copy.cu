@@ -5,7 +5,8 @@
 // Nothing is computed: the bound is the memory's copy rate, twice the bytes that move.  A block moves up to 16 KB (slots)
 // or one head's part of one layer's page (pages); a thread has four 16-byte loads in flight before its first store.  The
 // pairs travel as kernel arguments, so that nothing has to be brought to the device first.  Sources are never
-// destinations (the caller's rule, checked there), so blocks may run in any order.
+// destinations (the caller's rule, checked there), so blocks may run in any order.  The next kernel is not let go early: attention
+// kernels read pages that "earlier steps" have filled before they wait, and a copied page is one of those.
 #include "common.cuh"
 
 #define FORK_PAIRS 256
@@ -24,7 +25,6 @@ __global__ void __launch_bounds__(FORK_THREADS)
 TL_NAME(copy_slots_kernel)(unsigned char* __restrict__ storage, const __grid_constant__ ForkPairs p, long long layer_bytes,
                            long long row_bytes) {
   pdl_wait();
-  pdl_launch_dependents();
   unsigned char* layer = storage + (size_t)blockIdx.z * layer_bytes;
   const V* src = reinterpret_cast<const V*>(layer + (size_t)p.src[blockIdx.y] * row_bytes);
   V* dst = reinterpret_cast<V*>(layer + (size_t)p.dst[blockIdx.y] * row_bytes);
@@ -48,7 +48,6 @@ TL_NAME(copy_pages_kernel)(T* __restrict__ storage, const __grid_constant__ Fork
                            int heads, int dim, int vdim) {
   constexpr int W = 16 / sizeof(T);                 // numbers in 16 bytes
   pdl_wait();
-  pdl_launch_dependents();
   const int head = blockIdx.x, c = p.count[blockIdx.y], tid = threadIdx.x;
   T* layer = storage + (size_t)blockIdx.z * layer_elems;
   const size_t from = (size_t)p.src[blockIdx.y] * heads + head, to = (size_t)p.dst[blockIdx.y] * heads + head;

@@ -8,4 +8,5 @@ from . import attention_f32  # noqa: F401
 from . import moe_bf16  # noqa: F401
 from . import latent_bf16  # noqa: F401
 from . import attention_bf16  # noqa: F401
+from . import attention_shared  # noqa: F401
 from . import sink_attention_bf16  # noqa: F401
