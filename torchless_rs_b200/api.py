@@ -14,6 +14,7 @@ from typing import Callable, List, Optional, Sequence, Union
 import torch
 
 from .config import load_config
+from .engine.beam import BeamResult, generate_beams as _generate_beams
 from .engine.engine import Engine
 from .engine.generate import GenerationResult, generate as _generate
 from .engine.model import expected_tensors
@@ -72,6 +73,15 @@ class Model:
         self.engine = engine
         self._sampler = None
         self._reader = None
+        self._beam_selector = None
+
+    @property
+    def beam_selector(self):
+        """Built at first use, as the sampler."""
+        if self._beam_selector is None:
+            from .sampling.beam import BeamSelector
+            self._beam_selector = BeamSelector(self.engine.rt.device)
+        return self._beam_selector
 
     @property
     def sampler(self):
@@ -98,8 +108,27 @@ class Model:
         self.engine.check_kernels()
         return results
 
-    def step(self, slots, tokens, want="last"):
-        return self.engine.step(slots, tokens, want)
+    def generate_beams(self, prompts: Sequence[Sequence[int]], max_tokens: int = 16, beams: int = 4,
+                       length_penalty: float = 1.0, stop_ids: Optional[Sequence[int]] = None, n_best: int = 1,
+                       early_stop: bool = False, max_batch: Optional[int] = None) -> List[BeamResult]:
+        """Beam search: the `n_best` likeliest continuations of each prompt that a search of `beams` beams finds
+        (engine/beam.py has the rules).  `stop_ids` defaults to the configuration's end tokens; pass () for none.
+        The cache has to have `beams` sequence slots per prompt of a batch; the beams share the prompt's pages."""
+        if stop_ids is None:
+            stop_ids = self.engine.spec.stop_token_ids
+
+        def select(logits, scores, n):
+            on_device = torch.tensor(scores, dtype=torch.float32).to(logits.device)
+            out = self.beam_selector.ops.select(logits, on_device, n).cpu()
+            return out[0].view(torch.float32), out[1], out[2]
+
+        results = _generate_beams(self.engine, select, prompts, max_tokens, beams, length_penalty, stop_ids, n_best, early_stop,
+                                  max_batch=max_batch)
+        self.engine.check_kernels()
+        return results
+
+    def step(self, slots, tokens, want="last", groups=None):
+        return self.engine.step(slots, tokens, want, groups=groups)
 
     def prefill(self, slots, prompts, tokens_per_step=None):
         """The logits at each prompt's last token; many tokens go in several steps."""
@@ -114,6 +143,14 @@ class Model:
     def truncate(self, slot: int, length: int) -> None:
         """Rolls the sequence of `slot` back to its first `length` tokens."""
         self.engine.truncate(slot, length)
+
+    def fork(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Each held slot dst[i] goes on as a copy of the sequence of src[i]: pages are held together, state is copied."""
+        self.engine.fork(src, dst)
+
+    def reorder(self, slots: Sequence[int], parents: Sequence[int]) -> List[int]:
+        """Place j goes on from the sequence at place parents[j]; returns the slots in the new order."""
+        return self.engine.reorder(slots, parents)
 
     def reset(self, slot: int) -> None:
         """Rolls the sequence of `slot` back to empty; the slot stays held."""

@@ -16,6 +16,10 @@ advances (src/model/mod.rs:93).  Here many sequences live at once:
   the first `keep_first` positions are never given back while the sequence lives;
 * a state group holds [layers, slots, *shape], zeroed when a slot is taken.
 
+A sequence may go on from where another one stands (`fork`): it then holds the same pages, each of which knows how many
+sequences hold it, and a copy of the state.  A page that several hold is never written: the step that would write to it
+gives its sequence a page of its own with the positions so far (`prepare`).
+
 All decisions are taken on the host; the device only sees the page tables.
 """
 from __future__ import annotations
@@ -69,6 +73,7 @@ class PagedGroup:
         self.layers = list(layers)
         self.n_pages = n_pages
         self.pool = FreeList(n_pages, "cache page")
+        self.holders = np.zeros(n_pages, dtype=np.int32)   # sequences that hold a page
         if isinstance(request, PagedLatentRequest):
             shape = (len(self.layers), n_pages, PAGE * request.width)
         else:
@@ -103,9 +108,78 @@ class PagedGroup:
                 f"({self.table_host.shape[1] * PAGE})")
         got = self.pool.take(need)
         c = self.n_cols[slot]
+        self.holders[got] = 1
         self.table_host[slot, c:c + need] = got
         self.n_cols[slot] = c + need
         self._dirty.add(slot)
+
+    def _drop(self, pages) -> None:
+        """One sequence less holds each of these pages; those that none holds any more go back."""
+        pages = [int(p) for p in pages if p >= 0]
+        self.holders[pages] -= 1
+        self.pool.give_back(p for p in pages if self.holders[p] == 0)
+
+    def fork(self, src: int, dst: int) -> None:
+        """The slot `dst` lets go of what it holds and holds the pages of `src` from now on."""
+        c = self.n_cols[dst]
+        self._drop(self.table_host[dst, :c])
+        self.table_host[dst] = self.table_host[src]
+        held = self.table_host[src, :self.n_cols[src]]
+        self.holders[held[held >= 0]] += 1
+        self.first_live[dst], self.n_cols[dst] = self.first_live[src], self.n_cols[src]
+        self._dirty.add(dst)
+
+    def writes_into_shared(self, slots: Sequence[int], lengths: Sequence[int]) -> List[int]:
+        """Which of `slots` (indices into the list) need a page of their own before they write position lengths[i]: their last page is
+        begun and several hold it.  Of sequences that hold one page together, the last need not copy it if no other holds it."""
+        out, left = [], {}
+        for i, (s, n) in enumerate(zip(slots, lengths)):
+            if n % PAGE == 0:
+                continue
+            page = int(self.table_host[s, n // PAGE])
+            holders = left.get(page, int(self.holders[page]))
+            if holders > 1:
+                out.append(i)
+                left[page] = holders - 1
+        return out
+
+    def unshare(self, slots: Sequence[int], lengths: Sequence[int]) -> None:
+        """Gives each of `slots` a page of its own in the place of the page of position lengths[i], with the positions before it."""
+        if not slots:
+            return
+        cols = [n // PAGE for n in lengths]
+        src = [int(self.table_host[s, c]) for s, c in zip(slots, cols)]
+        dst = self.pool.take(len(slots))
+        for s, c, old, new in zip(slots, cols, src, dst):
+            self.holders[old] -= 1
+            self.holders[new] = 1
+            self.table_host[s, c] = new
+            self._dirty.add(s)
+        self.copy_pages(src, dst, [n % PAGE for n in lengths])
+
+    def copy_pages(self, src: Sequence[int], dst: Sequence[int], counts: Sequence[int]) -> None:
+        """The first counts[i] positions of page src[i] into page dst[i], in all layers."""
+        r = self.request
+        latent = isinstance(r, PagedLatentRequest)
+        heads, dim, vdim = (1, r.width, 0) if latent else (r.num_kv_heads, r.head_dim, r.value_dim)
+        if self.storage.is_cuda:
+            from ..csrc import ops
+            ops.core_ops(self.storage.dtype).copy_pages(self.storage.view(len(self.layers), -1), self.n_pages, heads, dim, vdim, src, dst, counts)
+            return
+        for layer in self.layers:              # (bookkeeping without a device)
+            view = self.view(layer)
+            for a, b, c in zip(src, dst, counts):
+                if latent:
+                    view.pages[b, :c] = view.pages[a, :c]
+                else:
+                    view.k_pages[b, :, :c] = view.k_pages[a, :, :c]
+                    view.v_pages[b, :, :, :c] = view.v_pages[a, :, :, :c]
+
+    def common_columns(self, slots: Sequence[int]) -> int:
+        """The leading columns in which the tables of `slots` agree."""
+        rows = self.table_host[list(slots), :max(self.n_cols[s] for s in slots)]
+        differ = np.flatnonzero((rows != rows[0]).any(axis=0))
+        return int(differ[0]) if len(differ) else rows.shape[1]
 
     def trim(self, slot: int, next_pos: int) -> None:
         """Gives back the pages that no position >= next_pos can see any more."""
@@ -118,7 +192,7 @@ class PagedGroup:
         if keep_from > f:
             lo = max(f, self.kept_cols)      # columns below hold the kept first positions
             if keep_from > lo:
-                self.pool.give_back(int(p) for p in self.table_host[slot, lo:keep_from])
+                self._drop(self.table_host[slot, lo:keep_from])
                 self.table_host[slot, lo:keep_from] = -1
                 self._dirty.add(slot)
             self.first_live[slot] = keep_from
@@ -138,7 +212,7 @@ class PagedGroup:
         f, c = self.first_live[slot], self.n_cols[slot]
         if keep >= c:
             return
-        self.pool.give_back(int(p) for p in self.table_host[slot, keep:c] if p >= 0)
+        self._drop(self.table_host[slot, keep:c])
         self.table_host[slot, keep:c] = -1
         self.n_cols[slot] = keep
         self.first_live[slot] = min(f, keep)
@@ -146,7 +220,7 @@ class PagedGroup:
 
     def release(self, slot: int) -> None:
         c = self.n_cols[slot]
-        self.pool.give_back(int(p) for p in self.table_host[slot, :c] if p >= 0)
+        self._drop(self.table_host[slot, :c])
         self.table_host[slot, :c] = -1
         self.first_live[slot] = 0
         self.n_cols[slot] = 0
@@ -201,6 +275,14 @@ class StateGroup:
 
     def reset(self, slot: int) -> None:
         self.storage[:, slot].zero_()
+
+    def fork(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """The state of each slot dst[i] becomes that of src[i], in all layers."""
+        if self.storage.is_cuda:
+            from ..csrc import ops
+            ops.core_ops(torch.float32).copy_slots(self.storage, src, dst)     # (bytes: the state's type does not matter)
+        else:
+            self.storage[:, list(dst)] = self.storage[:, list(src)]
 
     def view(self, layer: int) -> torch.Tensor:
         """[slots, *shape] of one layer."""
@@ -324,10 +406,61 @@ class Cache:
         """The sequence of `slot` starts again at its first token; the slot stays held."""
         self.truncate(slot, 0)
 
+    # ---- one sequence going on from another one's cache ----------------------------
+    def fork(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """The sequence of each held slot dst[i] ends and goes on as a copy of the sequence of src[i] (which may be a
+        source several times, and is no destination).  Pages are held together from then on, state is copied."""
+        src, dst = list(src), list(dst)
+        if len(src) != len(dst):
+            raise CacheStateError(f"{len(src)} sequences to copy and {len(dst)} slots for them")
+        for s in src + dst:
+            if not self.slots.is_held(s):
+                raise CacheStateError(f"sequence slot {s} is copied but is not held")
+        if len(set(dst)) != len(dst) or not set(dst).isdisjoint(src):
+            raise CacheStateError("a sequence slot is written twice, or both copied from and written")
+        if not src:
+            return
+        for g in self.paged:
+            for a, b in zip(src, dst):
+                g.fork(a, b)
+            g.upload()
+        for g in self.states:
+            g.fork(src, dst)
+        for a, b in zip(src, dst):
+            self.lengths[b] = self.lengths[a]
+
+    def reorder(self, slots: Sequence[int], parents: Sequence[int]) -> List[int]:
+        """What a beam search does between two steps: place j goes on from the sequence at place parents[j].  Returns the slots in
+        the new order.  A sequence that goes on keeps its slot in the first place that names it; the further
+        places get copies in the slots of sequences that nobody names, so the fewest copies are made."""
+        slots, parents = list(slots), list(parents)
+        if len(parents) != len(slots) or (parents and not 0 <= min(parents) <= max(parents) < len(slots)):
+            raise CacheStateError(f"{len(slots)} parents in [0, {len(slots)}) are needed, got {parents}")
+        if len(set(slots)) != len(slots):
+            raise CacheStateError("a sequence slot appears twice")
+        named = set(parents)
+        free = [s for j, s in enumerate(slots) if j not in named][::-1]
+        out, src, dst, seen = [], [], [], set()
+        for p in parents:
+            if p in seen:
+                src.append(slots[p])
+                dst.append(free.pop())
+                out.append(dst[-1])
+            else:
+                seen.add(p)
+                out.append(slots[p])
+        self.fork(src, dst)
+        return out
+
+    def common_columns(self, slots: Sequence[int]) -> int:
+        """The leading pages that the sequences of `slots` hold together, in every group of layers."""
+        return min((g.common_columns(slots) for g in self.paged), default=0)
+
     # ---- one step ----------------------------------------------------------------
     def prepare(self, slots: Sequence[int], new_lens: Sequence[int]) -> None:
-        """Makes room for each sequence to reach its new length and brings the
-        device's page tables up to date.  Nothing changes if there is no room."""
+        """Makes room for each sequence to reach its new length, gives a sequence that would write to a page
+        which others hold too a page of its own, and brings the device's page tables up to date.  Nothing
+        changes if there is no room."""
         for s in slots:
             if not self.slots.is_held(s):
                 raise CacheStateError(f"sequence slot {s} is used but is not held")
@@ -338,13 +471,16 @@ class Cache:
                 raise CacheCapacityError(
                     f"a sequence of {n} tokens is longer than the cache was sized for "
                     f"({self.max_seq_len})")
-        for g in self.paged:
-            need = sum(g.pages_needed(s, n) for s, n in zip(slots, new_lens))
+        past = [self.lengths[s] for s in slots]
+        copies = [g.writes_into_shared(slots, past) if g.pool.held_count else [] for g in self.paged]
+        for g, shared in zip(self.paged, copies):
+            need = sum(g.pages_needed(s, n) for s, n in zip(slots, new_lens)) + len(shared)
             if need > g.pool.free_count:
                 raise CacheCapacityError(
                     f"the cache is full: this step needs {need} more pages of {PAGE} tokens, "
                     f"{g.pool.free_count} of {g.n_pages} are free")
-        for g in self.paged:
+        for g, shared in zip(self.paged, copies):
+            g.unshare([slots[i] for i in shared], [past[i] for i in shared])
             for s, n in zip(slots, new_lens):
                 g.grow(s, n)
             g.upload()
@@ -376,17 +512,20 @@ class Cache:
         self.slots.check()
         for g in self.paged:
             g.pool.check()
-            seen = set()
+            seen: Dict[int, int] = {}
             for s in range(self.max_slots):
                 pages = [int(p) for p in g.table_host[s] if p >= 0]
                 if pages and not self.slots.is_held(s):
                     raise CacheStateError(f"free slot {s} still holds pages")
+                if len(set(pages)) != len(pages):
+                    raise CacheStateError(f"slot {s} holds a page twice")
                 for p in pages:
-                    if p in seen:
-                        raise CacheStateError(f"page {p} is in two places")
                     if not g.pool.is_held(p):
                         raise CacheStateError(f"page {p} is in a table but free")
-                    seen.add(p)
+                    seen[p] = seen.get(p, 0) + 1
+            for p, n in seen.items():
+                if n != g.holders[p]:
+                    raise CacheStateError(f"page {p} is in {n} places, held by {g.holders[p]}")
             if len(seen) != g.pool.held_count:
                 raise CacheStateError("a held page is in no table")
 

@@ -25,6 +25,10 @@ Options:
   --top-k <K>           Top-k sampling: only consider the top K tokens
   --top-p <P>           Nucleus sampling: keep smallest set of tokens with
                         cumulative probability >= P
+  --beams <N>           Beam search with N beams instead of sampling (then none of
+                        --temperature, --top-k, --top-p)
+  --length-penalty <P>  With --beams: hypotheses rank by log-probability divided by
+                        their length to the power of P (default: 1.0)
   --backend <BACKEND>   Compute backend: auto or cuda (the only one here)
   --dtype <TYPE>        bfloat16 (default) or float32 (true 32-bit everywhere)
   --seed <S>            Seed of the sampling draws (default: 0)
@@ -88,8 +92,8 @@ class CliError(Exception):
 
 
 def parse_args(argv: List[str]) -> dict:
-    opts = dict(max_tokens=None, max_seq_len=None, temperature=0.7, top_k=None, top_p=None,
-                dtype="bfloat16", seed=0, stop=(), debug=False, help=False, positional=[],
+    opts = dict(max_tokens=None, max_seq_len=None, temperature=None, top_k=None, top_p=None, beams=None,
+                length_penalty=None, dtype="bfloat16", seed=0, stop=(), debug=False, help=False, positional=[],
                 random_weights=False, weights_seed=0, save_weights=False)
     i = 0
 
@@ -117,6 +121,10 @@ def parse_args(argv: List[str]) -> dict:
             opts["top_k"] = value(a, int)
         elif a == "--top-p":
             opts["top_p"] = value(a, float)
+        elif a == "--beams":
+            opts["beams"] = value(a, int)
+        elif a == "--length-penalty":
+            opts["length_penalty"] = value(a, float)
         elif a == "--dtype":
             opts["dtype"] = value(a, str)
         elif a == "--seed":
@@ -143,6 +151,16 @@ def parse_args(argv: List[str]) -> dict:
         else:
             opts["positional"].append(a)
         i += 1
+    if opts["beams"] is not None:
+        if opts["beams"] < 1:
+            raise CliError("Error: --beams must be at least 1")
+        for name in ("temperature", "top_k", "top_p"):
+            if opts[name] is not None:
+                raise CliError(f"Error: --beams searches and does not sample: --{name.replace('_', '-')} does not go with it")
+    elif opts["length_penalty"] is not None:
+        raise CliError("Error: --length-penalty goes with --beams")
+    if opts["temperature"] is None:
+        opts["temperature"] = 0.7
     return opts
 
 
@@ -189,6 +207,11 @@ def main(argv: Optional[List[str]] = None, prog: str = "torchless") -> int:
         return 1
     max_tokens = min(max_tokens, max_seq_len - longest + 1)
     per_seq = (min(max_seq_len, longest + max_tokens) + 63) // 64 * 64
+    rows = len(prompts)
+    if opts["beams"]:
+        from .engine.beam import held_pages
+        per_seq = held_pages(longest, max_tokens, opts["beams"]) * 64
+        rows *= opts["beams"]
     if opts["debug"]:
         print(f"Loading {model_dir} ({opts['dtype']}), {len(prompts)} prompt(s), "
               f"max_tokens {max_tokens}, max_seq_len {max_seq_len}", file=sys.stderr)
@@ -202,11 +225,11 @@ def main(argv: Optional[List[str]] = None, prog: str = "torchless") -> int:
                 write_random_model(config, model_dir, opts["weights_seed"], api.parse_dtype(opts["dtype"]),
                                    "cuda:0")
             model = api.from_random(config, seed=opts["weights_seed"], dtype=opts["dtype"],
-                                    max_tokens=per_seq * len(prompts), max_batch=len(prompts),
+                                    max_tokens=per_seq * len(prompts), max_batch=rows,
                                     max_seq_len=max_seq_len)
         else:
             model = api.load(model_dir, dtype=opts["dtype"], max_tokens=per_seq * len(prompts),
-                             max_batch=len(prompts), max_seq_len=max_seq_len)
+                             max_batch=rows, max_seq_len=max_seq_len)
     except Exception as e:
         print(f"Error: {e}", file=sys.stderr)
         return 1
@@ -218,10 +241,18 @@ def main(argv: Optional[List[str]] = None, prog: str = "torchless") -> int:
             sys.stdout.write(f"{tok} ")
             sys.stdout.flush()
 
-    results = model.generate(prompts, max_tokens=max_tokens, temperature=opts["temperature"],
-                             top_k=opts["top_k"], top_p=opts["top_p"], stop_ids=stop,
-                             seed=opts["seed"], on_token=on_token)
-    if single:
+    if opts["beams"]:
+        try:
+            results = model.generate_beams(prompts, max_tokens=max_tokens, beams=opts["beams"], stop_ids=stop,
+                                           length_penalty=1.0 if opts["length_penalty"] is None else opts["length_penalty"])
+        except ValueError as e:
+            print(f"Error: {e}", file=sys.stderr)
+            return 1
+    else:
+        results = model.generate(prompts, max_tokens=max_tokens, temperature=opts["temperature"],
+                                 top_k=opts["top_k"], top_p=opts["top_p"], stop_ids=stop,
+                                 seed=opts["seed"], on_token=on_token)
+    if single and not opts["beams"]:
         sys.stdout.write("\n")
     else:
         for r in results:

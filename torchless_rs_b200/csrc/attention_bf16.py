@@ -9,6 +9,7 @@ from typing import Dict
 import torch
 
 from . import build
+from .attention_shared import run_shared
 from .ops import KernelError, _check, _need, _ptr, _stream, register_error_word
 
 FAST_HEAD_DIMS = (32, 64, 128)
@@ -261,6 +262,9 @@ class AttentionBf16:
     def run(self, q, cache_view, out, batch, nh, nkv, window, scale, workspace) -> bool:
         if self.lib is None or nh // nkv > MAX_GROUP:
             return False
+        if batch.is_decode and getattr(batch, "groups", None) is not None and \
+                run_shared(q, cache_view, out, batch, nh, nkv, window, scale, workspace):
+            return True
         if batch.is_decode:
             tma = getattr(self, "_decode_tma", None) is not None
             n_splits, quantum = decode_plan(batch.n_seqs, nkv, batch.len_bucket, window,

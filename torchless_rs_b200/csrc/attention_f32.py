@@ -8,6 +8,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import build
+from .attention_shared import run_shared
 from .ops import KernelError, _check, _need, _stream
 
 build.register_library("attn_f32", ("attention_f32.cu",), ())
@@ -112,6 +113,9 @@ class AttentionF32:
     def run(self, q: torch.Tensor, cache_view, out: torch.Tensor, batch, nh: int, nkv: int, window, scale: float,
             workspace) -> bool:
         hd = q.shape[1] // nh
+        if batch.is_decode and getattr(batch, "groups", None) is not None and \
+                run_shared(q, cache_view, out, batch, nh, nkv, window, scale, workspace):
+            return True
         if not batch.is_decode:
             if not self._tiles(batch, q.shape[0] * nh, nh, nkv, hd, window, q.device):
                 return False

@@ -160,3 +160,16 @@ class SharedAttention:
         rest = (window or 0, scale, splits, quantum, tails, _stream())
         _check(self._call(*head, *rest) if self.dtype == torch.bfloat16 else self._call(*head, hd, *rest), "attn_shared")
         _check(0, "attn_shared_merge")
+
+
+def run_shared(q, cache_view, out, batch, nh: int, nkv: int, window, scale: float, workspace) -> bool:
+    """A decode step whose rows hold leading pages together (`batch.groups`).  False where no kernel takes it: the caller
+    then uses one that reads every row's pages for itself."""
+    kernel = SharedAttention.get(q.dtype, q.shape[1] // nh)
+    if kernel is None or not kernel.takes(nh, nkv):
+        return False
+    g, c = batch.groups, cache_view
+    seen = min(batch.len_bucket, window + PAGE) if window else batch.len_bucket
+    kernel.decode(q, c.k_pages, c.v_pages, out, batch.seq_len, batch.seq_slot, c.page_table, g.start, g.pages, nh, nkv, window, scale,
+                  workspace, lens=g.lens, shared=g.shared, group_rows=max(g.rows), bound=-(-seen // PAGE))
+    return True

@@ -7,6 +7,25 @@ from typing import List, Optional, Sequence
 import numpy as np
 import torch
 
+from ..csrc.build import PAGE_TOKENS
+
+
+@dataclass
+class RowGroups:
+    """Consecutive rows of a decode step whose sequences have one length and hold their leading pages together (the beams of a
+    search).  On the host: `rows` of each group, its length after the step, the pages in common; on the device (int32) `start`
+    [groups + 1] and `pages` [groups]."""
+    rows: List[int]
+    lens: List[int]
+    shared: List[int]
+    start: Optional[torch.Tensor] = None
+    pages: Optional[torch.Tensor] = None
+
+    def key(self) -> tuple:
+        """What a recorded decode step assumes about its groups."""
+        own = max((-(-n // PAGE_TOKENS) - c for n, c in zip(self.lens, self.shared)), default=0)
+        return (tuple(self.rows), total_bucket([c * PAGE_TOKENS for c in self.shared]), 1 << max(own - 1, 0).bit_length())
+
 
 @dataclass
 class StepBatch:
@@ -37,6 +56,7 @@ class StepBatch:
     new_lens: List[int]
     token_src: Optional[torch.Tensor] = None   # device int32: tokens selected by the previous step
     total_bucket: Optional[int] = None           # the sum of the sequences' lengths after this step, rounded up
+    groups: Optional[RowGroups] = None           # rows that hold leading pages together (decode steps)
     plans: dict = field(default_factory=dict)    # which kernels the step's lengths call for, as layers find it out
 
 
@@ -92,6 +112,8 @@ class BatchStager:
     FIELDS = ("tokens", "token_seq", "token_pos", "seq_slot", "seq_start", "seq_len", "want_rows",
               "token_from")
 
+    GROUP_FIELDS = ("group_start", "group_pages")     # staged behind the others where a step has groups
+
     RING = 4   # pinned buffers in rotation, so the host can prepare a step while earlier copies run
 
     def __init__(self, device: torch.device):
@@ -141,8 +163,13 @@ class BatchStager:
             len_bucket=length_bucket(max_len), total_bucket=total_bucket(new_lens),
             slots=list(slots), past_lens=list(past_lens), new_lens=list(new_lens), **views)
 
-    def stage(self, arrays: dict, slots, past_lens, is_decode: bool) -> StepBatch:
-        sizes = [int(arrays[f].shape[0]) for f in self.FIELDS]
+    def stage(self, arrays: dict, slots, past_lens, is_decode: bool, groups: Optional[RowGroups] = None) -> StepBatch:
+        fields = self.FIELDS
+        if groups is not None:
+            fields = self.FIELDS + self.GROUP_FIELDS
+            arrays = dict(arrays, group_start=np.cumsum([0] + groups.rows, dtype=np.int32),
+                          group_pages=np.asarray(groups.shared, dtype=np.int32))
+        sizes = [int(arrays[f].shape[0]) for f in fields]
         offs, total = self._offsets(sizes)
         self._ensure(max(total, 1))
         self.staged += 1
@@ -151,14 +178,16 @@ class BatchStager:
             self.events[self.turn].synchronize()   # the copy that last used this buffer is done
         host = self.hosts[self.turn]
         hv = host.numpy()
-        for f, o, s in zip(self.FIELDS, offs, sizes):
+        for f, o, s in zip(fields, offs, sizes):
             hv[o:o + s] = arrays[f]
         self.dev[:total].copy_(host[:total], non_blocking=True)
         self.bytes_copied += 4 * total
         ev = self.events[self.turn] or torch.cuda.Event()
         ev.record()
         self.events[self.turn] = ev
-        views = {f: self.dev[o:o + s] for f, o, s in zip(self.FIELDS, offs, sizes)}
+        views = {f: self.dev[o:o + s] for f, o, s in zip(fields, offs, sizes)}
+        if groups is not None:
+            groups.start, groups.pages = views.pop("group_start"), views.pop("group_pages")
         counts = np.diff(arrays["seq_start"])
         max_len = int(arrays["seq_len"].max()) if sizes[5] else 0
         return StepBatch(
@@ -167,4 +196,4 @@ class BatchStager:
             max_len=max_len, len_bucket=length_bucket(max_len),
             total_bucket=total_bucket([int(x) for x in arrays["seq_len"]]),
             slots=list(slots), past_lens=list(past_lens),
-            new_lens=[int(x) for x in arrays["seq_len"]], **views)
+            new_lens=[int(x) for x in arrays["seq_len"]], groups=groups, **views)

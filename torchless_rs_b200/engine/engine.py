@@ -16,7 +16,7 @@ from ..cache import Cache
 from ..config.spec import ModelSpec
 from ..csrc import ops
 from ..parts.runtime import Runtime
-from .batch import BatchStager, StepBatch, layout_step, length_bucket, total_bucket
+from .batch import BatchStager, RowGroups, StepBatch, layout_step, length_bucket, total_bucket
 from .model import DecoderModel
 
 
@@ -72,6 +72,14 @@ class Engine:
         stays held."""
         self.cache.reset(slot)
 
+    def fork(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Each held slot dst[i] goes on as a copy of the sequence of src[i] (`Cache.fork`)."""
+        self.cache.fork(src, dst)
+
+    def reorder(self, slots: Sequence[int], parents: Sequence[int]) -> List[int]:
+        """Place j goes on from the sequence at place parents[j]; returns the slots in the new order (`Cache.reorder`)."""
+        return self.cache.reorder(slots, parents)
+
     def h2d_bytes(self) -> int:
         """Host-to-device bytes that steps have copied so far: step layouts and page-table rows."""
         return self.stager.bytes_copied + sum(g.bytes_copied for g in self.cache.paged)
@@ -84,7 +92,7 @@ class Engine:
     # ---- the step ----------------------------------------------------------------------
     def step(self, slots: Sequence[int], tokens: Optional[Sequence[Sequence[int]]] = None,
              want: Union[str, Sequence[Sequence[int]]] = "last",
-             from_device=None) -> Optional[torch.Tensor]:
+             from_device=None, groups: Optional[Sequence[int]] = None) -> Optional[torch.Tensor]:
         """Runs `tokens[b]` as the next tokens of the sequence in `slots[b]` and
         returns the 32-bit logits [wanted, vocab] on the device, in the order of the
         sequences and of their wanted places (`want[b]`: indices into `tokens[b]`;
@@ -93,8 +101,14 @@ class Engine:
 
         `from_device` = (source, indices) instead of `tokens`: every sequence goes on by the
         one token source[indices[b]], where `source` is an int32 tensor on the device (the
-        tokens a sampler selected).  The host then need not know the tokens to launch the step."""
+        tokens a sampler selected).  The host then need not know the tokens to launch the step.
+
+        `groups`: numbers of consecutive rows that went on from one sequence (the beams of each prompt).  In a decode step
+        the pages that such rows hold together are then read once for all of them; the result does not depend
+        on it beyond rounding."""
         B = len(slots)
+        if groups is not None and (sum(groups) != B or (B and min(groups) < 1)):
+            raise ValueError(f"groups of {list(groups)} rows do not make up the {B} slots")
         if B == 0:
             return None
         token_src = None
@@ -120,7 +134,7 @@ class Engine:
         # only positions and lengths differ, by one, and a kernel advances them on the device; the
         # host lays nothing out and copies nothing but page-table rows that gained a page.
         steady_key = None
-        if token_src is not None and all(c == 1 for c in counts) and all(w == [0] for w in want):
+        if token_src is not None and groups is None and all(c == 1 for c in counts) and all(w == [0] for w in want):
             steady_key = (tuple(slots), tuple(int(i) for i in src_index), token_src.data_ptr())
             st = self._steady
             if st is not None and st[0] == steady_key and st[1] == self.stager.staged and \
@@ -161,12 +175,33 @@ class Engine:
         if toks.size and (toks.min() < 0 or toks.max() >= self.vocab_size):
             raise ValueError(f"token ids must lie in [0, {self.vocab_size})")
         self.cache.prepare(slots, new_lens)
-        batch = self.stager.stage(arrays, slots, past, is_decode=all(c == 1 for c in counts))
+        is_decode = all(c == 1 for c in counts)
+        batch = self.stager.stage(arrays, slots, past, is_decode, self._row_groups(slots, new_lens, groups) if is_decode else None)
         batch.token_src = token_src
         self._steady = (steady_key, self.stager.staged, batch) if steady_key is not None else None
         logits = self._forward(batch)
         self.cache.commit(slots, new_lens)
         return logits
+
+    def _row_groups(self, slots, new_lens, groups) -> Optional[RowGroups]:
+        """The groups of a step and the pages in common; None where no two rows have any."""
+        if groups is None:
+            return None
+        rows, lens, shared = [], [], []
+        at = 0
+        for n in groups:
+            ss, ls = slots[at:at + n], new_lens[at:at + n]
+            at += n
+            common = self.cache.common_columns(ss) if n > 1 and len(set(ls)) == 1 else 0
+            if common:
+                rows.append(n)
+                lens.append(ls[0])
+                shared.append(common)
+            else:                      # rows by themselves
+                rows += [1] * n
+                lens += list(ls)
+                shared += [0] * n
+        return RowGroups(rows, lens, shared) if any(shared) else None
 
     # Tokens per step beyond which a batch of prompts is fed in several steps: a bound on the workspace (a
     # step of 65,536 tokens at the layer sizes of Mistral NeMo 12B holds some 6 GB of activations), not a
@@ -223,7 +258,8 @@ class Engine:
         if not (self.use_graphs and batch.is_decode and self.model.graph_safe):
             return self.model.forward(batch)
         key = (batch.n_seqs, batch.n_want, batch.len_bucket, batch.total_bucket, self.rt.workspace.generation,
-               batch.tokens.data_ptr(), batch.token_src.data_ptr() if batch.token_src is not None else 0)
+               batch.tokens.data_ptr(), batch.token_src.data_ptr() if batch.token_src is not None else 0,
+               batch.groups.key() if batch.groups is not None else None)
         hit = self._graphs.get(key)
         if hit is not None:
             hit[0].replay()
