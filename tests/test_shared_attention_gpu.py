@@ -16,9 +16,9 @@ DEV = "cuda"
 
 class Setting:
     """Groups of `beams[g]` rows of length lens[g] whose tables agree in shared[g] columns; pages in random order, numbers that no row
-    sees are NaN."""
+    sees are `junk`."""
 
-    def __init__(self, dtype, nh, nkv, hd, beams, lens, shared, window=None, seed=0, spread=1.5, junk=float("nan"), pages_more=3):
+    def __init__(self, dtype, nh, nkv, hd, beams, lens, shared, window=None, seed=0, spread=1.5, junk=1e4, pages_more=3):
         g = torch.Generator(device=DEV).manual_seed(seed)
         self.dtype, self.nh, self.nkv, self.hd, self.window = dtype, nh, nkv, hd, window
         self.beams, self.lens, self.shared = list(beams), list(lens), list(shared)
@@ -75,6 +75,7 @@ class Setting:
         rows, G = len(self.table), self.nh // self.nkv
         out = torch.zeros((rows, self.nh, self.hd), dtype=torch.float64, device=DEV)
         mass = torch.zeros_like(out)
+        self.largest = 0.0
         for r, (row, n) in enumerate(zip(self.table, self.row_len)):
             lo = max(0, n - self.window) if self.window else 0
             if n == 0:
@@ -83,23 +84,26 @@ class Setting:
             page = torch.tensor(row, device=DEV)[places // PAGE]
             k, v = self.k[page, :, places % PAGE].double(), self.v[page, :, :, places % PAGE].double()     # [keys, nkv, hd]
             q = self.q[r].double().view(self.nkv, G, self.hd)
-            p = torch.softmax(torch.einsum("hgd,nhd->hgn", q, k) * self.scale, -1)
+            score = torch.einsum("hgd,nhd->hgn", q, k) * self.scale
+            self.largest = max(self.largest, score.abs().max().item())
+            p = torch.softmax(score, -1)
             out[r] = torch.einsum("hgn,nhd->hgd", p, v).reshape(self.nh, self.hd)
             mass[r] = torch.einsum("hgn,nhd->hgd", p, v.abs()).reshape(self.nh, self.hd)
         return out.reshape(rows, -1), mass.reshape(rows, -1)
 
     def check(self, got=None):
         """bfloat16: a weight is rounded by at most 2^-8 of it, so the sum by 2^-8 of the weighted sum of |v|; the result by 2^-8 of
-        it; 32-bit sums of at most 4096 terms and exponentials are off by less than 2^-12 of that sum together.  32 bits: scores of
-        up to 2^5 off by (head size + 2) 2^-24 of sums of 64-term products (at most 2^7 in all), so weights by 2^-24 * 2^7 * 8 and
-        sums of n terms by 2^-24 n^(1/2) of the sum: 2^-13 of it covers both."""
+        it; 32-bit sums of at most 4096 terms and exponentials are off by less than 2^-12 of that sum together.  32 bits: a score is a
+        sum of head size terms and one product more, each step rounded by at most 2^-24 of the largest |score| S there is, so off by
+        e = (head size + 2) 2^-24 S; weights are then off by a factor of at most exp(e) either way, in the weighted sum and in the sum, 2 e
+        together; sums of n <= 4096 weights add less than 2^-13 (2^-24 n^(1/2) and exp's own 2^-23)."""
         got = self.run() if got is None else got
         want, mass = self.plain()
         assert torch.isfinite(got).all()
         if self.dtype == torch.bfloat16:
             bound = mass * (2.0 ** -8 + 2.0 ** -12) + want.abs() * 2.0 ** -8 + 1e-30
         else:
-            bound = mass * 2.0 ** -13 + 1e-30
+            bound = mass * max(2.0 ** -13, 2 * (self.hd + 2) * 2.0 ** -24 * self.largest) + 1e-30
         over = ((got.double() - want).abs() / bound).max().item()
         assert over <= 1.0, over
 
@@ -110,8 +114,9 @@ HEADS = [(torch.bfloat16, 8, 2, 64), (torch.bfloat16, 8, 2, 128), (torch.float32
 @pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
 @pytest.mark.parametrize("lens,shared", [([1], [0]), ([64], [0]), ([65], [1]), ([64], [1]), ([129, 63], [1, 0]), ([200, 1000, 64, 7], [3, 15, 1, 0]),
                                          ([4000], [60]), ([300, 2500], [0, 30])])
-def test_lengths_and_common_pages(dtype, nh, nkv, hd, lens, shared):
-    Setting(dtype, nh, nkv, hd, [4] * len(lens), lens, shared, seed=sum(lens)).check()
+@pytest.mark.parametrize("junk", [1e4, float("nan"), float("inf")])
+def test_lengths_and_common_pages(dtype, nh, nkv, hd, lens, shared, junk):
+    Setting(dtype, nh, nkv, hd, [4] * len(lens), lens, shared, seed=sum(lens), junk=junk).check()
 
 
 @pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64), (torch.float32, 128)])
@@ -124,8 +129,9 @@ def test_heads_and_beams(dtype, hd, nh, nkv, beams):
 
 @pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
 @pytest.mark.parametrize("window", [1, 63, 64, 65, 200, 1000])
-def test_windows(dtype, nh, nkv, hd, window):
-    Setting(dtype, nh, nkv, hd, [3, 4, 2], [500, 64, 1111], [6, 0, 16], window=window, seed=window).check()
+@pytest.mark.parametrize("junk", [1e4, float("nan")])
+def test_windows(dtype, nh, nkv, hd, window, junk):
+    Setting(dtype, nh, nkv, hd, [3, 4, 2], [500, 64, 1111], [6, 0, 16], window=window, seed=window, junk=junk).check()
 
 
 @pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
@@ -134,6 +140,22 @@ def test_a_key_that_stands_out_on_either_side_of_every_border(dtype, nh, nkv, hd
     for j, window in ((0, None), (127, None), (128, None), (383, None), (399, None), (100, 300), (101, 300)):
         s = Setting(dtype, nh, nkv, hd, [4], [400], [6], window=window, seed=j)
         s.k[s.table[0][j // PAGE], :, j % PAGE] = (s.q[0, :hd] * 4).to(dtype) if j >= 400 - (window or 400) else float("nan")
+        s.check()
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+def test_scores_that_grow_from_page_to_page(dtype, nh, nkv, hd):
+    """Every page's scores lie far above the pages' before, by a few and by some hundred powers of two: references have to move."""
+    for step in (3.0, 40.0, 150.0):
+        s = Setting(dtype, nh, nkv, hd, [4, 2], [700, 200], [9, 1], seed=1)
+        q = s.q.view(-1, nh, hd)
+        q[:, :, 0] = 1.0
+        q[1, :, 0] = -1.0                    # one row sees them fall
+        s.k[:, :, :, 0] = 0.0
+        for row in s.table:
+            for c, page in enumerate(row):
+                if page >= 0:
+                    s.k[page, :, :, 0] = c * step / s.scale
         s.check()
 
 
@@ -149,6 +171,30 @@ def test_scores_far_apart_and_scale(dtype, nh, nkv, hd):
 
 
 @pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+def test_values_of_a_rows_own_pages_that_are_no_numbers_stay_with_it(dtype, nh, nkv, hd):
+    """One row's own keys and values are infinite or NaN: its result is no number, the others' are what they were."""
+    for lens, shared, j in (([300], [2], 130), ([300], [2], 299), ([200], [3], 199), ([130], [0], 5)):
+        s = Setting(dtype, nh, nkv, hd, [4] * len(lens), lens, shared, seed=j)
+        clean = s.run()
+        for bad in (float("nan"), float("inf")):
+            t = Setting(dtype, nh, nkv, hd, [4] * len(lens), lens, shared, seed=j)
+            t.v[t.table[1][j // PAGE], 0, 3, j % PAGE] = bad
+            got = t.run().view(4, nh, hd)
+            mine = got[1, :nh // nkv, 3]
+            assert not torch.isfinite(mine).any() and (torch.isnan(mine).all() or bad == float("inf"))
+            rest = got.clone()
+            rest[1, :nh // nkv, 3] = clean.view(4, nh, hd)[1, :nh // nkv, 3]
+            t.v.copy_(s.v)
+            t.check(rest.view(4, -1))
+            t.k[t.table[2][j // PAGE], 1, j % PAGE] = bad
+            got = t.run().view(4, nh, hd)
+            assert not torch.isfinite(got[2, nh // nkv:]).any()
+            got[2, nh // nkv:] = clean.view(4, nh, hd)[2, nh // nkv:]
+            t.k.copy_(s.k)
+            t.check(got.view(4, -1))
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
 def test_rows_of_length_zero_give_zero(dtype, nh, nkv, hd):
     s = Setting(dtype, nh, nkv, hd, [2, 3], [0, 77], [0, 1])
     got = s.run()
@@ -160,8 +206,9 @@ def test_rows_of_length_zero_give_zero(dtype, nh, nkv, hd):
 def test_every_way_of_cutting_gives_the_result(dtype, nh, nkv, hd, monkeypatch):
     from torchless_rs_b200.csrc import attention_shared
     s = Setting(dtype, nh, nkv, hd, [4, 3], [1000, 333], [12, 3], seed=8)
-    for plan in ((1, 1, 1), (1, 100, 1), (3, 4, 2), (12, 1, 4), (60, 1, 4), (2, 3, 62), (13, 2, 7)):
-        monkeypatch.setattr(attention_shared, "shared_plan", lambda *a, plan=plan: plan)
+    for row_blocks, parts, blocks in ((1, 160, 148), (1, 2, 148), (2, 3, 148), (4, 20, 7), (1, 5, 1), (3, 160, 500), (1, 9, 33)):
+        monkeypatch.setattr(attention_shared, "shared_plan", lambda *a, plan=(row_blocks, parts): plan)
+        monkeypatch.setattr(attention_shared, "_sm_count", lambda device, blocks=blocks: blocks)
         s.check()
 
 

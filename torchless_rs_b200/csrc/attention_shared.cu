@@ -5,450 +5,562 @@
 //   o[r, h] = sum_j p_j v[j, h'] / sum_j p_j,   p_j = exp(scale q[r, h] . k[j, h'] - max),   j in [len - window, len)
 //
 // Consecutive rows form groups.  The page tables of a group's rows agree in their first `group_pages[g]` columns, so those
-// keys and values are read once for all of them: a block takes some of these pages for the rows x query heads of
-// one group and kv head, as the rows of one product.  Other blocks take the pages that are a row's own.  Every block leaves, per row and head, a maximum, a
-// sum and a weighted sum; a second kernel merges them in the order of the keys.  What bounds this is the memory: a page
-// of head size 128 is 32 KB per kv head and takes an SM 0.75 us at the copy rate, in which its rows' products are done.
+// keys and values are read once for all of them.  A unit of work is a group and kv head: its rows times query heads (R of them, padded to
+// N = 16, 32 or 64; more rows take several units) against the shared pages and then each row's own.  On the fifth-generation
+// tensor cores keys take the 128 lanes and rows the columns, so that few rows cost little:
+//   S^T[128 keys, N]  = K . Q^T      two pages of keys, Q in shared memory, S^T in tensor memory (two buffers)
+//   softmax           a key and half of the columns per thread; a column's reference is the score of the first key that it sees and
+//                     moves only when another exceeds it by 2^60, so that a tile needs one barrier of four warps and no maxima; P^T rounded to bfloat16 (2^-9 of each weight) to shared memory
+//   O^T[hd, N]       += V^T . P^T    the transposed value slab as it lies in the cache, O^T in tensor memory
+// A row's own page is multiplied with all rows of the unit; the others' weights are zero there, as all weights of keys that are not seen
+// are.  Where such a value is no number (0 x NaN is NaN) the second kernel finds a result that is none and computes it again,
+// from the keys that the row sees alone.
 //
-// Pages come by TMA (128-byte swizzle) into a ring of three stages; each of the four warps takes 16 keys of a page for all
-// rows, with mma.m16n8k16 on fragments read from shared memory.  Contraction slots are mapped to whatever dimensions (K) or keys
-// (V) a 16-byte or 8-byte read delivers, the same for both operands.  Scores, sums and accumulators are 32-bit; the weights are
-// rounded to bfloat16 before the second product (2^-9 of each, as the decode attention's).  Head sizes 64 and 128.
+// The tiles of all units lie in one line, which the blocks (one per SM) cut into equal stretches: nobody waits for the longest
+// sequence, and loads run on across units.  A unit that lies in one stretch is written to `out`; pieces leave a maximum, a sum and a weighted
+// sum per row and head, and a second kernel merges them in the order of the keys.  What bounds this is the memory: a tile of head
+// size 128 is 64 KB and takes an SM 1.5 us at the copy rate; its softmax and products take about a third of that.
 //
 // Nothing is read before the wait for the kernels before: a page may have been copied by one of them.  Every wait on an mbarrier
-// is bounded; when a bound is hit the block records a code in tl_attn_shared_error and stops.
+// is bounded; when a bound is hit the block records a code in tl_attn_shared_error, waits (bounded) for its copies in flight, frees its tensor
+// memory and returns.
 #include <cuda.h>
 #include <stdlib.h>
 
 #include "attention_bf16_common.cuh"
-#include "per_device.cuh"
-#include "umma.cuh"
+#include "attention_shared.cuh"
 
-#include <map>
-#include <mutex>
-#include <tuple>
-
-#define SH_WARPS 4
-#define SH_STAGES 3
+#define SH_SOFT 256                                 // threads of the softmax: warps 0-3 the lower half of the columns, 4-7 the upper
+#define SH_THREADS (SH_SOFT + 64)                   // warp 8 TMA, warp 9 tcgen05.mma
 #define SH_KSUB (HEAD_DIM / 64)                     // 64-column boxes of a K slab
-#define SH_K_BYTES (PAGE * HEAD_DIM * 2)
-#define SH_V_BYTES (HEAD_DIM * PAGE * 2)
-#define SH_STAGE_BYTES (SH_K_BYTES + SH_V_BYTES)
+#define SH_PAGE_K (PAGE * HEAD_DIM * 2)
+#define SH_PAGE_V (HEAD_DIM * PAGE * 2)
 #define SH_STRIDE (HEAD_DIM + 2)                    // floats of a partial result: weighted sum, maximum, sum
-#define SH_SMEM (1024 + SH_STAGES * SH_STAGE_BYTES + 256)
-#define SH_MAX_PARTS 64
+#define SH_MAX_HEADS 16                             // query heads per key/value head
+// A column's reference is the score of the first key that it sees and moves when a score exceeds it by 2^60: weights of up to that,
+// their sums and products with values are far from 32 bits' ends, and rounding to bfloat16 is relative.
+#define SH_SLACK 60.0f
 
 __device__ int tl_attn_shared_error = 0;
 
-__device__ __forceinline__ bool sh_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code) {
-  return tl_mbar_wait(bar, parity, abort_flag, code, &tl_attn_shared_error);
+__device__ __forceinline__ bool sh_park(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code) {
+  return tl_mbar_park(bar, parity, abort_flag, code, &tl_attn_shared_error);
 }
 __device__ __forceinline__ void sh_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ uint4 sh_lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
+__device__ __forceinline__ float sh_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-__device__ __forceinline__ uint2 sh_lds64(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-  return v;
+__device__ __forceinline__ void sh_bar(int half) { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); }   // four softmax warps
+__device__ __forceinline__ void sh_async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// C columns of this thread's lane: 8 at a time
+template <int C>
+__device__ __forceinline__ void sh_tmem_ld(uint32_t taddr, float (&v)[C]) {
+  static_assert(C % 8 == 0, "");
+#pragma unroll
+  for (int c = 0; c < C; c += 8)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[c]), "=f"(v[c + 1]), "=f"(v[c + 2]), "=f"(v[c + 3]), "=f"(v[c + 4]), "=f"(v[c + 5]), "=f"(v[c + 6]), "=f"(v[c + 7])
+                 : "r"(taddr + c));
+  tmem_ld_wait();
+  // (the values are there from here on, whatever order the compiler would like)
+#pragma unroll
+  for (int c = 0; c < C; ++c) asm volatile("" : "+f"(v[c]));
+}
+__device__ __forceinline__ void sh_tmem_st8(uint32_t taddr, const float* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+               "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ void sh_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ constexpr uint32_t sh_idesc(int n) {   // bf16 x bf16 -> f32, M = 128, both K-major
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-struct ShArgs {
-  const __nv_bfloat16* q;      // [rows][nh][HEAD_DIM]
-  float* part;                 // [rows][nh][parts][SH_STRIDE]
-  const int* seq_len;
-  const int* seq_slot;
-  const int* page_table;
-  const int* group_start;      // [groups + 1]
-  const int* group_pages;      // [groups]
-  int table_stride, nh, nkv, window;
-  float scale_log2;
-  int splits, quantum;         // of the shared pages: blocks, and the pages of each (the last takes what is left)
-  int tails;                   // blocks for the pages of a row's own
-  int row_blocks, beams;       // blocks that share the rows of a group, the group's rows of each
+// A weight at its place of P^T, by an address of shared memory (no clobber: the loop's loads and arithmetic may run past it).
+__device__ __forceinline__ void sh_store_bf16(uint32_t addr, float v) {
+  const unsigned short b = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+  asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(b));
+}
+
+// Bits c0 to c1 - 1.
+__device__ __forceinline__ uint32_t sh_mask(int c0, int c1) {
+  return (uint32_t)(((1ull << c1) - 1ull) & ~((1ull << c0) - 1ull));
+}
+// s <- s scale - reference in the columns that see this thread's key, -inf in the others; returns the largest.
+template <bool MASKED, int N>
+__device__ __forceinline__ float sh_shift(float (&s)[N], uint32_t columns, const float (&neg_ref)[N], float scale) {
+  float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    s[c] = fmaf(s[c], scale, neg_ref[c]);
+    if (MASKED) s[c] = (columns >> c & 1u) ? s[c] : -INFINITY;
+    if (c & 1) m1 = fmaxf(m1, s[c]); else m0 = fmaxf(m0, s[c]);
+  }
+  return fmaxf(m0, m1);
+}
+
+// Joins v[0 .. N) over the lanes of a warp into out[0 .. N): each exchange halves the columns that a lane holds.
+template <int N, typename F>
+__device__ __forceinline__ void sh_columns(const float (&v)[N], int lane, float* out, F join) {
+  float x[N / 2];
+  {
+    const bool up = (lane & 16) != 0;
+#pragma unroll
+    for (int c = 0; c < N / 2; ++c) {
+      const float send = up ? v[c] : v[c + N / 2], keep = up ? v[c + N / 2] : v[c];
+      x[c] = join(keep, __shfl_xor_sync(0xffffffffu, send, 16));
+    }
+  }
+  int cnt = N / 2;
+#pragma unroll
+  for (int mask = 8; mask > 0; mask >>= 1) {
+    const bool up = (lane & mask) != 0;
+    if (cnt > 1) {
+      cnt >>= 1;
+#pragma unroll
+      for (int c = 0; c < N / 4; ++c)
+        if (c < cnt) {
+          const float send = up ? x[c] : x[c + cnt], keep = up ? x[c + cnt] : x[c];
+          x[c] = join(keep, __shfl_xor_sync(0xffffffffu, send, mask));
+        }
+    } else {
+      x[0] = join(x[0], __shfl_xor_sync(0xffffffffu, x[0], mask));
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < (N >= 32 ? N / 32 : 1); ++c) out[lane * N / 32 + c] = x[c];
+}
+
+template <int N>
+struct ShSizes {
+  static constexpr int KS = HEAD_DIM == 64 ? (N == 64 ? 4 : 6) : (N == 64 ? 2 : 3), VS = HEAD_DIM == 64 ? 4 : 2;   // ring slots of two pages
+  static constexpr int K = 2 * SH_PAGE_K, V = 2 * SH_PAGE_V, Q = N * HEAD_DIM * 2, P = 2 * N * 128;
+  static constexpr int aux = SH_MAX_GROUPS * (int)sizeof(ShGroup) + 9 * N * 4 + 512;
+  static constexpr int smem = KS * K + VS * V + 2 * Q + 2 * P + aux;
+  static constexpr uint32_t tmem = N == 16 ? 64 : N == 32 ? 128 : 256;                             // S^T twice, O^T
 };
 
-// R8: eights of rows (rows of the group times query heads) that a block holds: 1, 2 or 4.
-template <int R8>
-__global__ void __launch_bounds__(SH_WARPS * 32, 2)
-FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const ShArgs a) {
-  constexpr int MT = (R8 + 1) / 2;
-  constexpr bool HI = R8 > 1;
-  extern __shared__ uint8_t sh_smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)sh_smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* full_bar = (uint64_t*)(smem + SH_STAGES * SH_STAGE_BYTES);
-  uint64_t* empty_bar = full_bar + SH_STAGES;
-  volatile int* abort_flag = (volatile int*)(empty_bar + SH_STAGES);
-  // the merge of the four warps reuses the stages after the loop
-  float* sm_o = (float*)smem;                                   // [warps][16 * MT][HEAD_DIM]
-  float* sm_m = sm_o + SH_WARPS * 16 * MT * HEAD_DIM;           // [warps][16 * MT]
-  float* sm_l = sm_m + SH_WARPS * 16 * MT;
+template <int N>
+__global__ void __launch_bounds__(SH_THREADS, 1)
+FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const ShArgs<__nv_bfloat16> a) {
+  using Z = ShSizes<N>;
+  // Swizzled tiles need 1024-byte alignment, which dynamic shared memory has when there is no static one (checked below).
+  extern __shared__ __align__(1024) uint8_t sh_smem[];
+  uint8_t* k_s = sh_smem;
+  uint8_t* v_s = k_s + Z::KS * Z::K;
+  uint8_t* q_s = v_s + Z::VS * Z::V;                   // [2][Q]
+  uint8_t* p_s = q_s + 2 * Z::Q;                       // [2][P]
+  ShGroup* table = (ShGroup*)(p_s + 2 * Z::P);
+  float* red_s = (float*)(table + SH_MAX_GROUPS);      // [4][N]
+  float* new_s = red_s + 4 * N;                        // [2][N]: scores of the first keys that columns see, by page of the tile
+  float* ref_s = new_s + 2 * N;                        // [N]
+  float* neg_s = ref_s + N;                            // [N]: the negated references, 0 for a column that has none
+  float* al_s = neg_s + N;                             // [N]
+  uint64_t* k_full = (uint64_t*)(al_s + N);
+  uint64_t* k_empty = k_full + Z::KS;
+  uint64_t* v_full = k_empty + Z::KS;
+  uint64_t* v_empty = v_full + Z::VS;
+  uint64_t* s_full = v_empty + Z::VS;                  // [2]
+  uint64_t* p_full = s_full + 2;                       // [2]
+  uint64_t* pv_done = p_full + 2;                      // [2]
+  uint64_t* q_full = pv_done + 2;                      // [2]
+  uint64_t* o_free = q_full + 2;
+  uint32_t* tmem_slot = (uint32_t*)(o_free + 1);
+  int* total_s = (int*)(tmem_slot + 1);                // [2]: tiles in the line, tiles of the longest unit
+  volatile int* abort_flag = (volatile int*)(total_s + 2);
+  // [2][3]: a reference in this half of the columns has to move.  By tile number modulo 3: written before a tile's barrier, read after
+  // it, cleared behind the next one (what a warp that runs ahead writes by then is another tile's).
+  volatile int* moved_s = abort_flag + 1;
 
-  const int kvh = blockIdx.y, grp = blockIdx.z;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
-  const int G = a.nh / a.nkv, parts = a.splits + a.tails;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < SH_STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], SH_WARPS); }
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (smem_u32(sh_smem) & 1023u) {                     // nothing has been allocated yet
+    if (tid == 0) atomicCAS(&tl_attn_shared_error, 0, 9);
+    return;
+  }
+  if (tid == 0) {
+    for (int s = 0; s < Z::KS; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
+    for (int s = 0; s < Z::VS; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
+    for (int u = 0; u < 2; ++u) {
+      mbar_init(&s_full[u], 1);
+      mbar_init(&p_full[u], SH_SOFT);
+      mbar_init(&pv_done[u], 1);
+      mbar_init(&q_full[u], SH_SOFT);
+    }
+    for (int u = 0; u < 6; ++u) moved_s[u] = 0;
+    mbar_init(o_free, SH_SOFT);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  __syncthreads();
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, Z::tmem);
+    tmem_relinquish();
+  }
   pdl_wait();
   pdl_launch_dependents();
+  if (warp == 8) sh_make_line<2>(table, total_s, a, lane);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot, tmem_o = tmem + 2 * N;
+  const int total = total_s[0], share = sh_share(total_s, gridDim.x, a.parts);
+  const int t0 = min((int)blockIdx.x * share, total), t1 = min(t0 + share, total);
+  const int G = a.nh / a.nkv;
 
-  // ---- which rows and which pages
-  const int g0 = a.group_start[grp], group_rows = a.group_start[grp + 1] - g0;
-  const int shared_blocks = a.splits * a.row_blocks;
-  const bool shared = (int)blockIdx.x < shared_blocks;
-  int row0, n_beams, slot;
-  if (shared) {
-    const int rb = blockIdx.x % a.row_blocks;
-    slot = blockIdx.x / a.row_blocks;
-    row0 = g0 + rb * a.beams;
-    n_beams = min(a.beams, group_rows - rb * a.beams);
-  } else {
-    const int y = blockIdx.x - shared_blocks;
-    row0 = g0 + y / a.tails;
-    n_beams = y / a.tails < group_rows ? 1 : 0;
-    slot = a.splits + y % a.tails;
-  }
-  if (n_beams <= 0) return;
-  const int R = n_beams * G;                 // rows of this block's products
-  const int len = a.seq_len[row0];           // of all rows of the group
-  const int lo = (a.window > 0 && len - a.window > 0) ? len - a.window : 0;
-  const int* table = a.page_table + (size_t)a.seq_slot[row0] * a.table_stride;
-  const int first = lo / PAGE, end = (len + PAGE - 1) / PAGE;      // columns that hold seen keys
-  const int border = min(max(a.group_pages[grp], first), end);     // columns before it are shared
-  int ps, pe;
-  if (shared) {
-    ps = first + slot * a.quantum;
-    pe = slot == a.splits - 1 ? border : min(ps + a.quantum, border);
-  } else {
-    const int per = (end - border + a.tails - 1) / a.tails;
-    ps = border + (slot - a.splits) * per;
-    pe = min(ps + per, end);
-  }
-  const int n_pg = max(0, pe - ps);
-  auto part_of = [&](int r) {      // row r of this block: its partial result
-    return a.part + (((size_t)(row0 + r / G) * a.nh + kvh * G + r % G) * parts + slot) * SH_STRIDE;
-  };
-  if (n_pg == 0) {                 // nothing here: a sum of zero marks it
-    for (int r = threadIdx.x; r < R; r += SH_WARPS * 32) {
-      float* dst = part_of(r);
-      dst[HEAD_DIM] = -INFINITY;
-      dst[HEAD_DIM + 1] = 0.0f;
-    }
-    return;
-  }
-
-  // one thread requests pages; `issue(i)` brings page ps + i into stage i % SH_STAGES
-  auto issue = [&](int i) {
-    const int s = i % SH_STAGES;
-    if (!sh_wait(&empty_bar[s], ((uint32_t)(i / SH_STAGES) & 1u) ^ 1u, abort_flag, 1)) return;
-    const int slab = table[ps + i] * a.nkv + kvh;
-    uint8_t* st = smem + (size_t)s * SH_STAGE_BYTES;
-    mbar_expect_tx(&full_bar[s], SH_STAGE_BYTES);
+  if (t0 < t1) {
+    if (warp == 8 && elect_one()) {
+      // ---- TMA: keys, then values, of every tile of the stretch
+      bool ok = true;
+      int n = 0;
+      for (int t = t0; t < t1 && ok;) {
+        const ShPiece p = sh_locate<2>(table, a, t);
+        const int last = min(p.tiles, p.tile + t1 - t);
+        for (int j = p.tile; j < last && ok; ++j, ++t, ++n) {
+          const int pages = min(2, p.pages - 2 * j);
+          int slab[2];
+          for (int h = 0; h < pages; ++h) {
+            int owner, col;
+            sh_page(p, 2 * j + h, owner, col);
+            slab[h] = a.page_table[(size_t)a.seq_slot[p.row0 + max(owner, 0)] * a.table_stride + col] * a.nkv + p.kvh;
+          }
+          const int ks = n % Z::KS, vs = n % Z::VS;
+          ok = sh_park(&k_empty[ks], ((uint32_t)(n / Z::KS) & 1u) ^ 1u, abort_flag, 1);
+          if (!ok) break;
+          mbar_expect_tx(&k_full[ks], pages * SH_PAGE_K);
+          for (int h = 0; h < pages; ++h)
 #pragma unroll
-    for (int sub = 0; sub < SH_KSUB; ++sub)
-      tma_load_2d(st + sub * (PAGE * 128), &tm_k, &full_bar[s], sub * 64, slab * PAGE);
-    tma_load_2d(st + SH_K_BYTES, &tm_v, &full_bar[s], 0, slab * HEAD_DIM);
-  };
-  if (threadIdx.x == 0)
-    for (int i = 0; i < SH_STAGES - 1 && i < n_pg; ++i) issue(i);
-
-  // query fragments
-  uint32_t qa[MT][NCHUNK][4], qb[MT][NCHUNK][4];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int ra = mt * 16 + g, rb = ra + 8;
-    const __nv_bfloat16* pa = a.q + ((size_t)(row0 + ra / G) * a.nh + kvh * G + ra % G) * HEAD_DIM;
-    const __nv_bfloat16* pb = a.q + ((size_t)(row0 + rb / G) * a.nh + kvh * G + rb % G) * HEAD_DIM;
-#pragma unroll
-    for (int j = 0; j < NCHUNK; ++j) {
-      uint4 va = make_uint4(0, 0, 0, 0), vb = make_uint4(0, 0, 0, 0);
-      if (ra < R) va = ldg16(pa + (4 * j + t) * 8);
-      if (HI && rb < R) vb = ldg16(pb + (4 * j + t) * 8);
-      qa[mt][j][0] = va.x; qa[mt][j][1] = va.y; qa[mt][j][2] = va.z; qa[mt][j][3] = va.w;
-      qb[mt][j][0] = vb.x; qb[mt][j][1] = vb.y; qb[mt][j][2] = vb.z; qb[mt][j][3] = vb.w;
-    }
-  }
-  float o[MT][NDT][4], m[MT][2], l[MT][2];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-    for (int i = 0; i < NDT; ++i) o[mt][i][0] = o[mt][i][1] = o[mt][i][2] = o[mt][i][3] = 0.0f;
-    m[mt][0] = m[mt][1] = -INFINITY;
-    l[mt][0] = l[mt][1] = 0.0f;
-  }
-
-  for (int i = 0; i < n_pg; ++i) {
-    if (threadIdx.x == 0 && i + SH_STAGES - 1 < n_pg) issue(i + SH_STAGES - 1);
-    __syncwarp();
-    const int s = i % SH_STAGES;
-    if (!sh_wait(&full_bar[s], (uint32_t)(i / SH_STAGES) & 1u, abort_flag, 2)) break;
-    const uint32_t kb = smem_u32(smem + (size_t)s * SH_STAGE_BYTES);
-    const uint32_t vb_ = kb + SH_K_BYTES;
-    const int key0 = (ps + i) * PAGE + 16 * warp;   // first of this warp's 16 keys
-    const bool whole = key0 >= lo && key0 + 16 <= len;
-    // ---- scores: 2 tiles of 8 keys; column c of tile jt is key 4*(c>>1) + 2*jt + (c&1)
-    float sc[MT][2][4];
-#pragma unroll
-    for (int jt = 0; jt < 2; ++jt) {
-      const int r = 16 * warp + 4 * (g >> 1) + 2 * jt + (g & 1);   // row of the K slab
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) sc[mt][jt][0] = sc[mt][jt][1] = sc[mt][jt][2] = sc[mt][jt][3] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < NCHUNK; ++j) {
-        const int chunk = 4 * j + t;
-        const uint4 kv = sh_lds128(kb + (uint32_t)(chunk >> 3) * (PAGE * 128) + (uint32_t)r * 128 +
-                                   (uint32_t)(((chunk & 7) ^ (r & 7)) << 4));
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          uint32_t f[4];
-          f[0] = qa[mt][j][0]; f[1] = qb[mt][j][0]; f[2] = qa[mt][j][1]; f[3] = qb[mt][j][1];
-          mma_bf16(sc[mt][jt], f, kv.x, kv.y);
-          f[0] = qa[mt][j][2]; f[1] = qb[mt][j][2]; f[2] = qa[mt][j][3]; f[3] = qb[mt][j][3];
-          mma_bf16(sc[mt][jt], f, kv.z, kv.w);
+            for (int sub = 0; sub < SH_KSUB; ++sub)
+              tma_load_2d(k_s + ks * Z::K + sub * (2 * PAGE * 128) + h * (PAGE * 128), &tm_k, &k_full[ks], sub * 64, slab[h] * PAGE);
+          ok = sh_park(&v_empty[vs], ((uint32_t)(n / Z::VS) & 1u) ^ 1u, abort_flag, 2);
+          if (!ok) break;
+          mbar_expect_tx(&v_full[vs], pages * SH_PAGE_V);
+          for (int h = 0; h < pages; ++h) tma_load_2d(v_s + vs * Z::V + h * SH_PAGE_V, &tm_v, &v_full[vs], 0, slab[h] * HEAD_DIM);
         }
       }
-    }
-    // ---- mask, running maximum, weights; column 2t+e of tile jt is key 4t + 2jt + e
-    uint32_t pa[MT][4];
-    float al[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-      for (int jt = 0; jt < 2; ++jt) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int idx = key0 + 4 * t + 2 * jt + e;
-          const bool ok = whole || (idx >= lo && idx < len);
-          sc[mt][jt][e] = ok ? sc[mt][jt][e] * a.scale_log2 : -INFINITY;
-          sc[mt][jt][2 + e] = ok ? sc[mt][jt][2 + e] * a.scale_log2 : -INFINITY;
-          mx0 = fmaxf(mx0, sc[mt][jt][e]);
-          mx1 = fmaxf(mx1, sc[mt][jt][2 + e]);
+      if (!ok) {
+        // given up: what is in flight lands before the block ends, or for as long as a wait may take
+        for (int i = 0; i < Z::KS && i < n; ++i)
+          for (uint32_t k = 0; k < TL_WAIT_LIMIT / 64 && !tl_mbar_try_wait(&k_full[(n - 1 - i) % Z::KS], (uint32_t)((n - 1 - i) / Z::KS) & 1u); ++k) {}
+        for (int i = 0; i < Z::VS && i < n; ++i)
+          for (uint32_t k = 0; k < TL_WAIT_LIMIT / 64 && !tl_mbar_try_wait(&v_full[(n - 1 - i) % Z::VS], (uint32_t)((n - 1 - i) / Z::VS) & 1u); ++k) {}
+        const int ks = n % Z::KS;    // the tile that was given up half way
+        for (uint32_t k = 0; k < TL_WAIT_LIMIT / 64 && !tl_mbar_try_wait(&k_full[ks], (uint32_t)(n / Z::KS) & 1u); ++k) {}
+      }
+    } else if (warp == 9 && elect_one()) {
+      // ---- the products: S^T of tile n + 1 before O^T of tile n
+      constexpr uint32_t idesc = sh_idesc(N);
+      const uint32_t desc_hi = (uint32_t)(smem_desc_k128(0) >> 32);
+      auto lo_of = [](const uint8_t* s) { return ((smem_u32(s) & 0x3FFFFu) >> 4) | (1u << 16); };
+      auto desc = [&](uint32_t lo) { return ((uint64_t)desc_hi << 32) | lo; };
+      const uint32_t k_lo = lo_of(k_s), v_lo = lo_of(v_s), q_lo = lo_of(q_s), p_lo = lo_of(p_s);
+      const int tiles = t1 - t0;
+      bool ok = true;
+      // tile n + 1's unit runs ahead of tile n's
+      int s_unit = 0, s_left = 0, s_t = t0;       // for S^T: units begun, tiles left of the current one
+      int o_unit = 0, o_left = 0, o_t = t0, o_tile = 0;
+      ShPiece o_piece = {};
+      bool o_first = false;
+      auto scores = [&](int n) {
+        if (s_left == 0) {
+          const ShPiece p = sh_locate<2>(table, a, s_t);
+          s_left = min(p.tiles - p.tile, t1 - s_t);
+          s_t += s_left;
+          if (!sh_park(&q_full[s_unit & 1], (uint32_t)(s_unit >> 1) & 1u, abort_flag, 3)) return false;
+          ++s_unit;
         }
+        --s_left;
+        if (!sh_park(&k_full[n % Z::KS], (uint32_t)(n / Z::KS) & 1u, abort_flag, 4)) return false;
+        tc_fence_after();
+        const uint32_t ka = k_lo + (uint32_t)(n % Z::KS) * (Z::K >> 4), qa = q_lo + (uint32_t)((s_unit - 1) & 1) * (Z::Q >> 4);
+#pragma unroll
+        for (int kk = 0; kk < HEAD_DIM / 16; ++kk)
+          umma_bf16(tmem + (uint32_t)(n & 1) * N, desc(ka + (kk >> 2) * ((2 * PAGE * 128) >> 4) + (kk & 3) * 2),
+                    desc(qa + (kk >> 2) * ((N * 128) >> 4) + (kk & 3) * 2), idesc, kk > 0 ? 1u : 0u);
+        umma_commit(&s_full[n & 1]);
+        umma_commit(&k_empty[n % Z::KS]);
+        return true;
+      };
+      ok = scores(0);
+      for (int n = 0; n < tiles && ok; ++n) {
+        if (n + 1 < tiles && !scores(n + 1)) break;     // (its buffer was read before P of tile n - 1 was there)
+        if (o_left == 0) {
+          o_piece = sh_locate<2>(table, a, o_t);
+          o_left = min(o_piece.tiles - o_piece.tile, t1 - o_t);
+          o_t += o_left;
+          o_tile = o_piece.tile;
+          o_first = true;
+          // O^T is free when the unit before has been written out
+          if (o_unit > 0 && !sh_park(o_free, (uint32_t)(o_unit - 1) & 1u, abort_flag, 5)) break;
+          ++o_unit;
+        }
+        if (!sh_park(&v_full[n % Z::VS], (uint32_t)(n / Z::VS) & 1u, abort_flag, 6) ||
+            !sh_park(&p_full[n & 1], (uint32_t)(n >> 1) & 1u, abort_flag, 7))
+          break;
+        tc_fence_after();
+        const uint32_t va = v_lo + (uint32_t)(n % Z::VS) * (Z::V >> 4), pa = p_lo + (uint32_t)(n & 1) * (Z::P >> 4);
+        const int pages = min(2, o_piece.pages - 2 * o_tile);
+        for (int h = 0; h < pages; ++h)        // a second page that is not there is not multiplied
+#pragma unroll
+          for (int kk = 0; kk < PAGE / 16; ++kk) {
+            umma_bf16(tmem_o, desc(va + h * (SH_PAGE_V >> 4) + kk * 2), desc(pa + h * ((N * 128) >> 4) + kk * 2), idesc, o_first ? 0u : 1u);
+            o_first = false;
+          }
+        umma_commit(&pv_done[n & 1]);
+        umma_commit(&v_empty[n % Z::VS]);
+        --o_left;
+        ++o_tile;
       }
-      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-      if (HI) {
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+    } else if (warp < 8) {
+      // ---- softmax: key `key` of a tile, columns first_col to first_col + NC - 1.  A wait that runs out leaves the loop's barriers in
+      // place: the warps go through them to the end (every later wait returns at once), and what they write is not valid.
+      constexpr int NC = N / 2;
+      const int upper = warp >> 2, key = tid & 127, page_of = key >> 6, first_col = upper * NC, quad = warp & 3;
+      const uint32_t t_lane = (uint32_t)(quad * 32) << 16;
+      volatile int* moved = moved_s + 3 * upper;
+      auto load_q = [&](const ShPiece& p, int buf) {
+        uint8_t* dst = q_s + buf * Z::Q;
+        for (int i = tid; i < N * (HEAD_DIM / 8); i += SH_SOFT) {
+          const int r = i / (HEAD_DIM / 8), c = i % (HEAD_DIM / 8);
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (r < p.beams * G) v = ldg16(a.q + ((size_t)(p.row0 + r / G) * a.nh + p.kvh * G + r % G) * HEAD_DIM + c * 8);
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * (N * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+        }
+        sh_async_fence();
+        sh_arrive(&q_full[buf]);
+      };
+      int n = 0, unit = 0;
+      float l[NC], neg_ref[NC];                // sums of this thread's weights; the negated references (0: none yet)
+      auto load_refs = [&] {
+#pragma unroll
+        for (int c = 0; c < NC; c += 4) {
+          const float4 r = *reinterpret_cast<const float4*>(neg_s + first_col + c);
+          neg_ref[c] = r.x; neg_ref[c + 1] = r.y; neg_ref[c + 2] = r.z; neg_ref[c + 3] = r.w;
+        }
+      };
+      ShPiece p = sh_locate<2>(table, a, t0);
+      load_q(p, 0);
+      for (int t = t0; t < t1; ++unit) {
+        const int last = min(p.tiles, p.tile + t1 - t), R = p.beams * G;
+        const int next = t + last - p.tile;
+        ShPiece np = p;
+        if (next < t1) {                       // the next unit's queries: its buffer's scores were all read a unit ago
+          np = sh_locate<2>(table, a, next);
+          load_q(np, (unit + 1) & 1);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) l[c] = neg_ref[c] = 0.0f;
+        if (key < NC) {
+          ref_s[first_col + key] = -INFINITY;
+          neg_s[first_col + key] = 0.0f;
+        }
+        sh_bar(upper);
+        const uint32_t all = sh_mask(0, min(max(R - first_col, 0), NC));
+        uint32_t is_set = 0;                   // columns that have a reference
+        // this thread's page of the tile, step by step
+        int owner = -1, in_own = 0, col = p.first + 2 * p.tile + page_of;
+        if (2 * p.tile + page_of >= p.common) {
+          owner = p.own ? (2 * p.tile + page_of - p.common) / p.own : 0;
+          in_own = 2 * p.tile + page_of - p.common - owner * p.own;
+          col = p.first + p.common + in_own;
+        }
+        for (int j = p.tile; j < last; ++j, ++n) {
+          const int buf = n & 1, now3 = n % 3;
+          const bool there = 2 * j + page_of < p.pages;
+          const uint32_t columns = owner < 0 ? all : sh_mask(min(max(owner * G - first_col, 0), NC), min(max(owner * G + G - first_col, 0), NC));
+          const int at = col * PAGE + (key & 63);
+          const bool seen = there && at >= p.lo && at < p.len;
+          const bool plain = there && owner < 0 && col * PAGE >= p.lo && col * PAGE + PAGE <= p.len;
+          sh_park(&s_full[buf], (uint32_t)(n >> 1) & 1u, abort_flag, 9);
+          tc_fence_after();
+          float s[NC];                         // scores, then weights
+          const uint32_t t_s = tmem + t_lane + (uint32_t)buf * N + first_col;
+          sh_tmem_ld<NC>(t_s, s);
+          if (is_set != all) {
+            // columns that see their first keys: the score of the first of them becomes the reference
+            uint32_t of[2] = {0u, 0u};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (2 * j + h >= p.pages) continue;
+              int ow, cl;
+              sh_page(p, 2 * j + h, ow, cl);
+              of[h] = (ow < 0 ? all : sh_mask(min(max(ow * G - first_col, 0), NC), min(max(ow * G + G - first_col, 0), NC))) & ~is_set;
+              if (of[h] && key == h * PAGE + max(p.lo - cl * PAGE, 0)) {
+#pragma unroll
+                for (int c = 0; c < NC; c += 4)
+                  *reinterpret_cast<float4*>(new_s + h * N + first_col + c) = make_float4(s[c], s[c + 1], s[c + 2], s[c + 3]);
+              }
+            }
+            of[1] &= ~of[0];
+            if (of[0] | of[1]) {
+              sh_bar(upper);
+              if (key < NC && (of[0] | of[1]) >> key & 1u) {
+                const float first = new_s[((of[0] >> key & 1u) ? 0 : N) + first_col + key];
+                const float ref = fmaxf(first * a.scale, -1e30f);
+                ref_s[first_col + key] = ref;
+                neg_s[first_col + key] = -ref;
+              }
+              sh_bar(upper);
+              load_refs();
+              is_set |= of[0] | of[1];
+            }
+          }
+          const float largest = plain ? sh_shift<false>(s, columns, neg_ref, a.scale) : sh_shift<true>(s, seen ? columns : 0u, neg_ref, a.scale);
+          if (__any_sync(0xffffffffu, largest > SH_SLACK) && lane == 0) moved[now3] = 1;
+          sh_bar(upper);
+          if (key == 0) moved[(n + 2) % 3] = 0;
+          if (moved[now3]) {
+            // another reference for the columns that need one: the maximum of this tile's scores
+            sh_tmem_ld<NC>(t_s, s);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) s[c] = seen && (columns >> c & 1u) ? s[c] * a.scale : -INFINITY;
+            sh_columns<NC>(s, lane, red_s + quad * N + first_col, [](float x, float y) { return fmaxf(x, y); });
+            sh_bar(upper);
+            if (key < NC) {
+              const float* r = red_s + first_col + key;
+              const float m = fmaxf(fmaxf(r[0], r[N]), fmaxf(r[2 * N], r[3 * N])), old = ref_s[first_col + key];
+              const float now = m > old + SH_SLACK ? m : old;
+              ref_s[first_col + key] = now;
+              neg_s[first_col + key] = now == -INFINITY ? 0.0f : -now;
+              al_s[first_col + key] = now == old ? 1.0f : sh_ex2(old - now);
+            }
+            sh_bar(upper);
+            load_refs();
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              l[c] *= al_s[first_col + c];
+              s[c] += neg_ref[c];
+            }
+            if (j > p.tile) {
+              // O^T so far, once the product before is done (the next one waits for this tile's weights)
+              sh_park(&pv_done[buf ^ 1], (uint32_t)((n - 1) >> 1) & 1u, abort_flag, 10);
+              tc_fence_after();
+              float o[NC];
+              sh_tmem_ld<NC>(tmem_o + t_lane + first_col, o);
+#pragma unroll
+              for (int c = 0; c < NC; ++c) o[c] *= al_s[first_col + c];
+#pragma unroll
+              for (int c = 0; c < NC; c += 8) sh_tmem_st8(tmem_o + t_lane + first_col + c, o + c);
+              sh_tmem_st_wait();
+            }
+          }
+          // weights; P^T of two tiles ago has been read
+          if (n >= 2) sh_park(&pv_done[buf], (uint32_t)((n - 2) >> 1) & 1u, abort_flag, 11);
+          const uint32_t pw = smem_u32(p_s + buf * Z::P + page_of * (N * 128) + first_col * 128), k2 = (uint32_t)(key & 63) * 2;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            s[c] = sh_ex2(s[c]);
+            l[c] += s[c];
+          }
+#pragma unroll
+          for (int c = 0; c < NC; ++c) sh_store_bf16(pw + c * 128 + (k2 ^ ((c & 7) << 4)), s[c]);
+          sh_async_fence();
+          tc_fence_before();
+          sh_arrive(&p_full[buf]);
+          // two pages on
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            ++col;
+            if (owner < 0) {
+              if (col == p.first + p.common) { owner = 0; in_own = 0; }
+            } else if (++in_own >= p.own) {
+              in_own = 0;
+              ++owner;
+              col = p.first + p.common;
+            }
+          }
+        }
+        // ---- the unit's end: sums over the keys, O^T out
+        sh_columns<NC>(l, lane, red_s + quad * N + first_col, [](float x, float y) { return x + y; });
+        sh_bar(upper);
+        const int first_block = p.start / share, pieces = (p.start + p.tiles - 1) / share - first_block + 1;
+        const int slot = (int)blockIdx.x - first_block;
+        if (tid == 0 && slot == 0) a.unit_parts[p.unit] = pieces;
+        // (What runs once per unit is fetched from afar, some ten cycles an instruction: it is written as loops, without divisions.)
+        const int my_r = first_col + key;
+        if (key < NC && my_r < R) {
+          const float sum = (red_s[my_r] + red_s[N + my_r]) + (red_s[2 * N + my_r] + red_s[3 * N + my_r]);
+          al_s[my_r] = pieces > 1 ? 1.0f : 1.0f / sum;
+          if (pieces > 1) {
+            const int beam = my_r / G;
+            float* dst = a.part + (((size_t)(p.row0 + beam) * a.nh + p.kvh * G + my_r - beam * G) * a.parts + slot) * SH_STRIDE + HEAD_DIM;
+            dst[0] = ref_s[my_r];
+            dst[1] = sum;
+          }
+        }
+        sh_bar(upper);
+        sh_park(&pv_done[(n - 1) & 1], (uint32_t)((n - 1) >> 1) & 1u, abort_flag, 13);
+        tc_fence_after();
+        if (key < HEAD_DIM) {                  // (whole warps)
+          int beam = first_col / G, g = first_col - beam * G;
+          size_t head = (size_t)(p.row0 + beam) * a.nh + p.kvh * G + g;
+#pragma unroll 1
+          for (int c = 0; c < NC && first_col + c < R; c += 8) {
+            float o[8];
+            sh_tmem_ld<8>(tmem_o + t_lane + first_col + c, o);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int r = first_col + c + e;
+              if (r < R) {
+                if (pieces > 1) a.part[(head * a.parts + slot) * SH_STRIDE + key] = o[e];
+                else a.out[head * HEAD_DIM + key] = __float2bfloat16_rn(o[e] * al_s[r]);
+              }
+              ++head;
+              if (++g == G) { g = 0; head += a.nh - G; }
+            }
+          }
+        }
+        tc_fence_before();
+        sh_arrive(o_free);
+        sh_bar(upper);                         // red_s and ref_s are written again
+        t = next;
+        p = np;
       }
-      const float n0 = fmaxf(m[mt][0], mx0), n1 = fmaxf(m[mt][1], mx1);
-      // the 16 keys of a warp may all lie outside the sequence or the window
-      const float ref0 = n0 == -INFINITY ? 0.0f : n0, ref1 = n1 == -INFINITY ? 0.0f : n1;
-      al[mt][0] = exp2f(m[mt][0] - ref0);
-      al[mt][1] = HI ? exp2f(m[mt][1] - ref1) : 0.0f;
-      m[mt][0] = n0;
-      m[mt][1] = n1;
-      float r0 = 0.0f, r1 = 0.0f;
-#pragma unroll
-      for (int jt = 0; jt < 2; ++jt) {
-        const float p0 = exp2f(sc[mt][jt][0] - ref0), p1 = exp2f(sc[mt][jt][1] - ref0);
-        const float p2 = HI ? exp2f(sc[mt][jt][2] - ref1) : 0.0f, p3 = HI ? exp2f(sc[mt][jt][3] - ref1) : 0.0f;
-        r0 += p0 + p1;
-        r1 += p2 + p3;
-        pa[mt][2 * jt] = pack_bf16(p0, p1);
-        pa[mt][2 * jt + 1] = pack_bf16(p2, p3);
-      }
-      l[mt][0] = l[mt][0] * al[mt][0] + r0;
-      l[mt][1] = l[mt][1] * al[mt][1] + r1;
-    }
-    // ---- o = o * alpha + p . v; thread (g, t) reads v^T[dim 8i + g][keys 16*warp + 4t .. +3].  Values of keys that
-    // are not seen stay out whatever they are (0 x NaN is NaN).
-    uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-    if (!whole) {
-      const int k = key0 + 4 * t;
-      keep0 = (k >= lo && k < len ? 0xffffu : 0u) | (k + 1 >= lo && k + 1 < len ? 0xffff0000u : 0u);
-      keep1 = (k + 2 >= lo && k + 2 < len ? 0xffffu : 0u) | (k + 3 >= lo && k + 3 < len ? 0xffff0000u : 0u);
-    }
-#pragma unroll
-    for (int i2 = 0; i2 < NDT; ++i2) {
-      const int row = 8 * i2 + g;
-      const uint2 vv = sh_lds64(vb_ + (uint32_t)row * 128 + (uint32_t)(((2 * warp + (t >> 1)) ^ (row & 7)) << 4) +
-                                (uint32_t)(t & 1) * 8);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        o[mt][i2][0] *= al[mt][0]; o[mt][i2][1] *= al[mt][0]; o[mt][i2][2] *= al[mt][1]; o[mt][i2][3] *= al[mt][1];
-        mma_bf16(o[mt][i2], pa[mt], vv.x & keep0, vv.y & keep1);
-      }
-    }
-    __syncwarp();
-    if (lane == 0) sh_arrive(&empty_bar[s]);
-  }
-
-  __syncthreads();   // every warp is done with the stages; unless a wait ran out, every requested page has arrived
-  if (*abort_flag) {
-    // no result; the block stays until its copies in flight have landed (a stage's last request is that of the last page
-    // with its number), or for as long as a wait may take
-    if (threadIdx.x == 0)
-      for (int i = max(0, n_pg - SH_STAGES); i < n_pg; ++i)
-        for (uint32_t k = 0; k < TL_WAIT_LIMIT / 64 && !tl_mbar_try_wait(&full_bar[i % SH_STAGES], (uint32_t)(i / SH_STAGES) & 1u); ++k) {}
-    __syncthreads();
-    return;
-  }
-  // ---- merge the four warps of the block (their keys are disjoint)
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 1);
-      l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 2);
     }
   }
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int base = warp * 16 * MT + mt * 16 + g;
-    if (t == 0) {
-      sm_m[base] = m[mt][0]; sm_l[base] = l[mt][0];
-      sm_m[base + 8] = m[mt][1]; sm_l[base + 8] = l[mt][1];
-    }
-#pragma unroll
-    for (int i = 0; i < NDT; ++i) {
-      float* ro = sm_o + (size_t)base * HEAD_DIM + 8 * i + 2 * t;
-      *reinterpret_cast<float2*>(ro) = make_float2(o[mt][i][0], o[mt][i][1]);
-      if (HI) *reinterpret_cast<float2*>(ro + 8 * HEAD_DIM) = make_float2(o[mt][i][2], o[mt][i][3]);
-    }
-  }
+  __syncwarp();
+  tc_fence_before();
   __syncthreads();
-  for (int idx = threadIdx.x; idx < R * HEAD_DIM; idx += SH_WARPS * 32) {
-    const int r = idx / HEAD_DIM, d = idx - r * HEAD_DIM;
-    float mm = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < SH_WARPS; ++w) mm = fmaxf(mm, sm_m[w * 16 * MT + r]);
-    float acc = 0.0f, ll = 0.0f;
-#pragma unroll
-    for (int w = 0; w < SH_WARPS; ++w) {
-      const float wm = sm_m[w * 16 * MT + r];
-      const float f = wm == -INFINITY ? 0.0f : exp2f(wm - mm);
-      acc += f * sm_o[(size_t)(w * 16 * MT + r) * HEAD_DIM + d];
-      ll += f * sm_l[w * 16 * MT + r];
-    }
-    float* dst = part_of(r);
-    dst[d] = acc;
-    if (d == 0) { dst[HEAD_DIM] = mm; dst[HEAD_DIM + 1] = ll; }
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Z::tmem);
   }
 }
 
-// Merges the partial results of one (row, head), a thread per dimension, in the order of the keys.  A row without any key
-// (of length 0) gives zero.
-__global__ void __launch_bounds__(HEAD_DIM)
-FN(attn_shared_merge_kernel)(const float* __restrict__ part, __nv_bfloat16* __restrict__ out, int nh, int parts) {
-  __shared__ float f_s[SH_MAX_PARTS], l_s[SH_MAX_PARTS];
-  pdl_wait();
-  pdl_launch_dependents();
-  const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
-  const float* src = part + ((size_t)b * nh + h) * parts * SH_STRIDE;
-  constexpr int AHEAD = 16;        // of the first parts this thread's number is fetched before their weights are known
-  float v[AHEAD];
-#pragma unroll
-  for (int s = 0; s < AHEAD; ++s) v[s] = s < parts ? src[s * SH_STRIDE + d] : 0.0f;
-  if (d < parts) {
-    f_s[d] = src[d * SH_STRIDE + HEAD_DIM];
-    l_s[d] = src[d * SH_STRIDE + HEAD_DIM + 1];
-  }
-  __syncthreads();
-  float m = -INFINITY;
-  for (int s = 0; s < parts; ++s) m = fmaxf(m, f_s[s]);
-  float acc = 0.0f, l = 0.0f;
-#pragma unroll
-  for (int s = 0; s < AHEAD; ++s) {
-    if (s < parts && l_s[s] != 0.0f) {       // (an empty part's weighted sum was never written)
-      const float f = exp2f(f_s[s] - m);
-      acc += f * v[s];
-      l += f * l_s[s];
-    }
-  }
-#pragma unroll 4
-  for (int s = AHEAD; s < parts; ++s) {
-    if (l_s[s] != 0.0f) {
-      const float f = exp2f(f_s[s] - m);
-      acc += f * src[s * SH_STRIDE + d];
-      l += f * l_s[s];
-    }
-  }
-  out[((size_t)b * nh + h) * HEAD_DIM + d] = __float2bfloat16_rn(l != 0.0f ? acc / l : 0.0f);
-}
-
-// ---------------------------------------------------------------------------
-// Host side
-// ---------------------------------------------------------------------------
-typedef CUresult (*ShEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// rows x cols bfloat16, contiguous rows; boxes of 64 columns (128 bytes) x box_rows, 128-byte swizzle.  What is kept by address is the
-// map, which is a function of the address and the sizes alone.
-static bool sh_make_map(CUtensorMap* map, const void* ptr, long long rows, long long cols, int box_rows) {
-  typedef std::tuple<const void*, long long, long long, int> Key;
-  static std::map<Key, CUtensorMap> cache;
-  static std::mutex mu;
-  static ShEncodeFn fn = nullptr;
-  std::lock_guard<std::mutex> lock(mu);
-  const Key key(ptr, rows, cols, box_rows);
-  auto it = cache.find(key);
-  if (it != cache.end()) { *map = it->second; return true; }
-  if (!fn) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
-      return false;
-    fn = (ShEncodeFn)p;
-  }
-  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
-  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUtensorMap m;
-  if (fn(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-    return false;
-  if (cache.size() > 4096) cache.clear();
-  cache[key] = m;
-  *map = m;
-  return true;
-}
-
-template <int R8>
-static int sh_run(const CUtensorMap& tk, const CUtensorMap& tv, const ShArgs& a, dim3 grid, cudaStream_t stream) {
-  const cudaError_t set = tl_allow_smem<FN(attn_shared_kernel)<R8>>(SH_SMEM);
+template <int N>
+static int sh_run(const CUtensorMap& tk, const CUtensorMap& tv, const ShArgs<__nv_bfloat16>& a, int blocks, cudaStream_t stream) {
+  constexpr int smem = ShSizes<N>::smem;
+  static_assert(smem <= 232448, "a block's shared memory");
+  const cudaError_t set = tl_allow_smem<FN(attn_shared_kernel)<N>>(smem);
   if (set != cudaSuccess) return (int)set;
-  return tl_launch(FN(attn_shared_kernel)<R8>, grid, dim3(SH_WARPS * 32), (size_t)SH_SMEM, stream, tk, tv, a);
+  return tl_launch(FN(attn_shared_kernel)<N>, dim3(blocks), dim3(SH_THREADS), (size_t)smem, stream, tk, tv, a);
 }
 
 // q, out [rows][nh][HEAD_DIM]; the rows of group g are group_start[g] to group_start[g + 1] - 1, at most `group_rows` of them, of one
-// length; `part`: rows * nh * (splits + tails) * (HEAD_DIM + 2) floats.  `splits`, `quantum`, `tails`: see ShArgs.
+// length.  `row_blocks`: units that a group's rows are split into, at most 64 / (nh / nkv) rows each; `part`: rows * nh * parts *
+// (HEAD_DIM + 2) floats, `parts` pieces of a unit at most (2 to 160); `unit_parts`: groups * row_blocks * nkv ints; `blocks`: blocks to launch.
 // Returns 0, a CUDA error, or -1 / -2 for arguments that are refused / sizes that are not taken.
 extern "C" int FN(tl_attn_shared)(const void* q, const void* k_pages, const void* v_pages, long long n_pages, void* out, float* part,
-                                  const int* seq_len, const int* seq_slot, const int* page_table, int table_stride,
+                                  int* unit_parts, const int* seq_len, const int* seq_slot, const int* page_table, int table_stride,
                                   const int* group_start, const int* group_pages, int groups, int rows, int group_rows, int nh, int nkv,
-                                  int window, float scale, int splits, int quantum, int tails, cudaStream_t stream) {
+                                  int window, float scale, int row_blocks, int parts, int blocks, cudaStream_t stream) {
   if (rows <= 0 || groups <= 0) return 0;
-  if (nkv <= 0 || nh <= 0 || nh % nkv || splits < 1 || quantum < 1 || tails < 1 || group_rows < 1 || window < 0) return -1;
-  const int G = nh / nkv;
-  if (G > 16 || splits + tails > SH_MAX_PARTS || nkv > 65535 || groups > 65535 || rows > 65535 ||
+  if (nkv <= 0 || nh <= 0 || nh % nkv || row_blocks < 1 || parts < 2 || blocks < 1 || group_rows < 1 || window < 0) return -1;
+  const int G = nh / nkv, beams = (group_rows + row_blocks - 1) / row_blocks, R = beams * G;
+  if (G > SH_MAX_HEADS || R > 64 || parts > SH_MAX_PARTS || groups > SH_MAX_GROUPS || nkv > 65535 || group_rows > 65535 ||
       n_pages * nkv * (HEAD_DIM > PAGE ? HEAD_DIM : PAGE) > 0x7fffffffLL || ((uintptr_t)q & 15) || ((uintptr_t)k_pages & 15) || ((uintptr_t)v_pages & 15))
     return -2;
   CUtensorMap tk, tv;
-  if (!sh_make_map(&tk, k_pages, n_pages * nkv * PAGE, HEAD_DIM, PAGE)) return -2;
-  if (!sh_make_map(&tv, v_pages, n_pages * nkv * HEAD_DIM, PAGE, HEAD_DIM)) return -2;
-  // as few blocks as hold a group's rows, 32 products' rows each, evenly
-  const int row_blocks = (group_rows * G + 32 / G * G - 1) / (32 / G * G), beams = (group_rows + row_blocks - 1) / row_blocks;
-  ShArgs a = {(const __nv_bfloat16*)q, part, seq_len, seq_slot, page_table, group_start, group_pages, table_stride, nh, nkv, window,
-              scale * 1.4426950408889634f, splits, quantum, tails, row_blocks, beams};
-  const dim3 grid(splits * row_blocks + group_rows * tails, nkv, groups);
-  const int R = beams * G;
-  const int st = R <= 8 ? sh_run<1>(tk, tv, a, grid, stream) : R <= 16 ? sh_run<2>(tk, tv, a, grid, stream) : sh_run<4>(tk, tv, a, grid, stream);
+  if (!sh_make_map(&tk, k_pages, n_pages * nkv * PAGE, HEAD_DIM, PAGE, 2)) return -2;
+  if (!sh_make_map(&tv, v_pages, n_pages * nkv * HEAD_DIM, PAGE, HEAD_DIM, 2)) return -2;
+  const ShArgs<__nv_bfloat16> a = {(const __nv_bfloat16*)q, (__nv_bfloat16*)out, part, unit_parts, seq_len, seq_slot, page_table, group_start, group_pages,
+                    table_stride, groups, nh, nkv, window, scale * 1.4426950408889634f, parts, row_blocks, beams};
+  const int st = R <= 16 ? sh_run<16>(tk, tv, a, blocks, stream) : R <= 32 ? sh_run<32>(tk, tv, a, blocks, stream) : sh_run<64>(tk, tv, a, blocks, stream);
   if (st) return st;
-  return tl_launch(FN(attn_shared_merge_kernel), dim3(nh, rows), dim3(HEAD_DIM), 0, stream, (const float*)part, (__nv_bfloat16*)out, nh,
-                   splits + tails);
+  return tl_launch(attn_shared_merge_kernel<HEAD_DIM, true, true, __nv_bfloat16>, dim3(nh, group_rows, groups), dim3(HEAD_DIM), 0, stream, a,
+                   (const __nv_bfloat16*)k_pages, (const __nv_bfloat16*)v_pages);
 }
 
 extern "C" int FN(tl_attn_shared_take_error)() {

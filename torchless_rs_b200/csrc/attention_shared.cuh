@@ -1,0 +1,284 @@
+// What the two forms of decode attention over shared pages have in common (attention_shared.cu, attention_shared_f32.cu): the units of
+// work, the line of their tiles that the blocks cut into equal stretches, the merge of a unit's pieces, tensor maps.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+#include "per_device.cuh"
+#include "umma.cuh"
+
+#include <map>
+#include <mutex>
+#include <tuple>
+
+#ifndef PAGE
+#define PAGE TL_PAGE
+#endif
+static_assert(PAGE == 64, "the tiles are laid out for pages of 64 tokens");
+
+#define SH_MAX_PARTS 160
+#define SH_MAX_GROUPS 256
+
+template <typename T>
+struct ShArgs {
+  const T* q;                  // [rows][nh][head size]
+  T* out;                      // the same
+  float* part;                 // [rows][nh][parts][head size + 2]: weighted sum, maximum, sum
+  int* unit_parts;             // [groups][row_blocks][nkv]: pieces of a unit
+  const int* seq_len;
+  const int* seq_slot;
+  const int* page_table;
+  const int* group_start;      // [groups + 1]
+  const int* group_pages;      // [groups]
+  int table_stride, groups, nh, nkv, window;
+  float scale;                 // (bfloat16: times log2 e)
+  int parts;                   // room for pieces of a unit
+  int row_blocks, beams;       // units that share the rows of a group, the group's rows of each
+};
+
+// The pages that the rows of a group see: `first` column, how many are common, how many are each row's own.
+struct ShSpan {
+  int len, lo, first, common, own;
+};
+__device__ __forceinline__ ShSpan sh_span(int len, int window, int shared) {
+  ShSpan s;
+  s.len = len;
+  s.lo = (window > 0 && len - window > 0) ? len - window : 0;
+  s.first = s.lo / PAGE;
+  const int end = (len + PAGE - 1) / PAGE, border = min(max(shared, s.first), end);
+  s.common = border - s.first;
+  s.own = end - border;
+  return s;
+}
+struct ShGroup {
+  int before;                  // tiles of the groups before
+  int row0, rows, len, lo, first, common, own;
+};
+// A stretch of a unit's tiles.
+struct ShPiece {
+  int kvh, row0, beams, len, lo, first, common, own, pages;
+  int tile, tiles;             // the first tile of the stretch, tiles of the unit
+  int unit, start;             // the unit's number, its first tile in the line
+};
+
+// TP: pages of a tile
+template <int TP>
+__device__ __forceinline__ int sh_tiles(int common, int own, int beams) { return (common + own * beams + TP - 1) / TP; }
+
+// One warp: the groups' places in the line.  totals: tiles in the line, tiles of the longest unit.
+template <int TP, typename T>
+__device__ __forceinline__ void sh_make_line(ShGroup* table, int* totals, const ShArgs<T>& a, int lane) {
+  int before = 0, longest = 0;
+  for (int g0 = 0; g0 < a.groups; g0 += 32) {
+    const int g = g0 + lane;
+    ShGroup e = {};
+    int n = 0;
+    if (g < a.groups) {
+      e.row0 = a.group_start[g];
+      e.rows = a.group_start[g + 1] - e.row0;
+      if (e.rows > 0) {
+        const ShSpan s = sh_span(a.seq_len[e.row0], a.window, a.group_pages[g]);
+        e.len = s.len; e.lo = s.lo; e.first = s.first; e.common = s.common; e.own = s.own;
+        const int full = e.rows / a.beams, rest = e.rows - full * a.beams;
+        n = a.nkv * (full * sh_tiles<TP>(s.common, s.own, a.beams) + (rest ? sh_tiles<TP>(s.common, s.own, rest) : 0));
+        longest = max(longest, sh_tiles<TP>(s.common, s.own, min(e.rows, a.beams)));
+      }
+    }
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    e.before = before + sum - n;
+    if (g < a.groups) table[g] = e;
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+  if (lane == 0) { totals[0] = before; totals[1] = longest; }
+}
+// The length of a stretch: an equal share, but no unit in more pieces than there is room for.
+__device__ __forceinline__ int sh_share(const int* totals, int blocks, int parts) {
+  return max((totals[0] + blocks - 1) / blocks, (totals[1] + parts - 2) / (parts - 1));
+}
+
+template <int TP, typename T>
+__device__ ShPiece sh_locate(const ShGroup* table, const ShArgs<T>& a, int t) {
+  int lo = 0, hi = a.groups - 1;
+  while (lo < hi) {            // the last group that begins at or before t and has tiles
+    const int mid = (lo + hi + 1) >> 1;
+    if (table[mid].before <= t) lo = mid; else hi = mid - 1;
+  }
+  const ShGroup& g = table[lo];
+  const int full = g.rows / a.beams, rest = g.rows - full * a.beams;
+  const int t_full = sh_tiles<TP>(g.common, g.own, a.beams), t_rest = rest ? sh_tiles<TP>(g.common, g.own, rest) : 0;
+  const int per_kv = full * t_full + t_rest, in_group = t - g.before, kvh = in_group / per_kv, r = in_group - kvh * per_kv;
+  const int rb = min(r / t_full, full), j = r - rb * t_full;
+  ShPiece p;
+  p.kvh = kvh;
+  p.row0 = g.row0 + rb * a.beams;
+  p.beams = rb < full ? a.beams : rest;
+  p.len = g.len; p.lo = g.lo; p.first = g.first; p.common = g.common; p.own = g.own;
+  p.pages = g.common + g.own * p.beams;
+  p.tile = j;
+  p.tiles = rb < full ? t_full : t_rest;
+  p.unit = (lo * a.row_blocks + rb) * a.nkv + kvh;
+  p.start = t - j;
+  return p;
+}
+// Page i of a unit: the row (of the unit) whose table and weights it takes, -1 for a common one, and the table's column.
+__device__ __forceinline__ void sh_page(const ShPiece& p, int i, int& owner, int& col) {
+  if (i < p.common) {
+    owner = -1;
+    col = p.first + i;
+  } else {
+    owner = (i - p.common) / p.own;
+    col = p.first + p.common + (i - p.common) - owner * p.own;
+  }
+}
+
+// Merges the pieces of one (row, head), a thread per dimension, in the order of the keys; a unit in one piece has been
+// written.  A row without any key (of length 0) gives zero.  EXP2: the maxima are logarithms to the base 2.
+//
+// AGAIN: a result that is no number is computed again from the keys that the row sees, one page after the other (the first kernel
+// multiplies values that it does not see by zero).  That is slow, and needed only where the cache holds values that are no numbers.
+template <int HD, bool EXP2, bool AGAIN, typename T>
+__global__ void __launch_bounds__(HD)
+attn_shared_merge_kernel(const ShArgs<T> a, const T* __restrict__ k_pages, const T* __restrict__ v_pages) {
+  __shared__ float f_s[SH_MAX_PARTS];
+  // what the call was given may be read before the wait: the kernel before this one has waited for those that wrote it
+  const int h = blockIdx.x, in_group = blockIdx.y, g = blockIdx.z, d = threadIdx.x, lane = d & 31;
+  const int row0 = a.group_start[g], row = row0 + in_group;
+  const bool there = row < a.group_start[g + 1];
+  const ShSpan span = sh_span(there ? a.seq_len[row0] : 0, a.window, a.group_pages[g]);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (!there) return;
+  const size_t head = (size_t)row * a.nh + h;
+  auto store = [&](float v) {
+    if constexpr (sizeof(T) == 2) a.out[head * HD + d] = __float2bfloat16_rn(v); else a.out[head * HD + d] = v;
+  };
+  if (span.common + span.own == 0) {
+    store(0.0f);
+    return;
+  }
+  const float* src = a.part + head * a.parts * (HD + 2);
+  constexpr int AHEAD = 8;         // of the first pieces this thread's number is fetched before it is known how many there are
+  float v[AHEAD];
+#pragma unroll
+  for (int s = 0; s < AHEAD; ++s) v[s] = s < a.parts ? src[s * (HD + 2) + d] : 0.0f;
+  const int kvh = h / (a.nh / a.nkv), parts = a.unit_parts[((size_t)g * a.row_blocks + in_group / a.beams) * a.nkv + kvh];
+  float result;
+  if (parts <= 1) {
+    if (!AGAIN) return;
+    result = to_f32(a.out[head * HD + d]);
+  } else {
+    // every warp: the largest reference, the factors, the sum (a piece in which this row sees no key has a reference of -inf)
+    constexpr int ROUNDS = (SH_MAX_PARTS + 31) / 32;
+    float ref[ROUNDS], sum[ROUNDS], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      const int s = lane + 32 * i;
+      ref[i] = s < parts ? src[s * (HD + 2) + HD] : -INFINITY;
+      sum[i] = s < parts ? src[s * (HD + 2) + HD + 1] : 0.0f;
+      m = fmaxf(m, ref[i]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      const float f = ref[i] == -INFINITY ? 0.0f : EXP2 ? exp2f(ref[i] - m) : expf(ref[i] - m);
+      l += f * sum[i];
+      if (d < 32 && lane + 32 * i < SH_MAX_PARTS) f_s[lane + 32 * i] = f;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    __syncthreads();
+    float acc = 0.0f;
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s)
+      if (s < parts) acc += f_s[s] * v[s];
+#pragma unroll 8
+    for (int s = AHEAD; s < parts; ++s) acc += f_s[s] * src[s * (HD + 2) + d];
+    result = acc / l;
+    store(result);
+  }
+  if constexpr (AGAIN) {
+    if (!__syncthreads_or(!isfinite(result))) return;
+    __shared__ float p_s[PAGE];
+    __shared__ float q_s[HD];
+    const int* table = a.page_table + (size_t)a.seq_slot[row] * a.table_stride;
+    const float scale = EXP2 ? a.scale * 0.6931471805599453f : a.scale;
+    q_s[d] = to_f32(a.q[head * HD + d]);
+    float m = -INFINITY, l = 0.0f, acc = 0.0f;
+    for (int col = span.first; col < span.first + span.common + span.own; ++col) {
+      const size_t slab = (size_t)table[col] * a.nkv + kvh;
+      const int from = max(span.lo - col * PAGE, 0), to = min(span.len - col * PAGE, PAGE);
+      __syncthreads();
+      for (int k = from + d; k < to; k += HD) {
+        const T* key = k_pages + (slab * PAGE + k) * HD;
+        float s = 0.0f;
+        for (int e = 0; e < HD; ++e) s = fmaf(q_s[e], to_f32(key[e]), s);
+        p_s[k] = s * scale;
+      }
+      __syncthreads();
+      float top = m;
+      for (int k = from; k < to; ++k) top = fmaxf(top, p_s[k]);
+      const float alpha = m == top ? 1.0f : expf(m - top);
+      m = top;
+      l *= alpha;
+      acc *= alpha;
+      const T* value = v_pages + (slab * HD + d) * PAGE;
+      for (int k = from; k < to; ++k) {
+        const float w = expf(p_s[k] - m);
+        l += w;
+        acc = fmaf(w, to_f32(value[k]), acc);
+      }
+    }
+    store(acc / l);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+typedef CUresult (*ShEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// rows x cols numbers of `size` bytes (2: bfloat16, 4: 32-bit), contiguous rows; boxes of 128 bytes x box_rows, 128-byte swizzle.  What is
+// kept by address is the map, which is a function of the address and the sizes alone.
+static bool sh_make_map(CUtensorMap* map, const void* ptr, long long rows, long long cols, int box_rows, int size) {
+  typedef std::tuple<const void*, long long, long long, int, int> Key;
+  static std::map<Key, CUtensorMap> cache;
+  static std::mutex mu;
+  static ShEncodeFn fn = nullptr;
+  std::lock_guard<std::mutex> lock(mu);
+  const Key key(ptr, rows, cols, box_rows, size);
+  auto it = cache.find(key);
+  if (it != cache.end()) { *map = it->second; return true; }
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      return false;
+    fn = (ShEncodeFn)p;
+  }
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)cols * size};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUtensorMap m;
+  if (fn(&m, size == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(ptr), dims, strides, box,
+         estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return false;
+  if (cache.size() > 4096) cache.clear();
+  cache[key] = m;
+  *map = m;
+  return true;
+}

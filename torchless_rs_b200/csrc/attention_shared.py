@@ -13,61 +13,37 @@ from .ops import KernelError, _check, _here, _need, _sm_count, _stream, register
 
 HEAD_DIMS = (64, 128)
 PAGE = build.PAGE_TOKENS
-MAX_PARTS = 64                 # partial results of a row and head that the merge takes
-BLOCK_ROWS = 32                # rows (of a group, times query heads) that one block holds
-MAX_GROUP = {torch.bfloat16: 16, torch.float32: 32}     # query heads per key/value head
+MAX_GROUPS = 256               # groups of one call
+MAX_HEADS = {torch.bfloat16: 16, torch.float32: 32}     # query heads per key/value head
+BLOCK_ROWS = {torch.bfloat16: 64, torch.float32: 32}    # rows of a unit (rows of a group, times query heads)
+TILE_PAGES = {torch.bfloat16: 2, torch.float32: 1}      # pages that a block takes at a time
+MAX_PARTS = 160                # pieces of a unit that the merge takes
 
 for _hd in HEAD_DIMS:
     build.register_library(f"attn_shared_bf16_hd{_hd}", ("attention_shared.cu",), (f"-DHEAD_DIM={_hd}",))
 build.register_library("attn_shared_f32", ("attention_shared_f32.cu",), ())
 
-# What the plan knows about the kernels (measured on a B200, head size 128)
-PAGE_US = {torch.bfloat16: 1.0, torch.float32: 2.8}     # a block alone, a page
-SETUP_US = 1.5                                          # a block's start and the write of its partial results
-MERGE_US, PART_US = 2.5, 0.03                           # the second kernel, and what every part adds to it
-HBM_GBS = 6500.0
-PER_SM = {torch.bfloat16: 2, torch.float32: 1}          # resident blocks
-
 
 @lru_cache(maxsize=4096)
-def shared_plan(lens: Tuple[int, ...], shared: Tuple[int, ...], group_rows: int, nkv: int, group: int, head_dim: int,
-                window: int, dtype: torch.dtype, sms: int, bound: int = 0) -> Tuple[int, int, int]:
-    """(splits, quantum, tails): blocks that share a group's common pages of one kv head and the pages of each, and blocks that
-    share a row's own pages.  `lens` and `shared` per group: length and pages in common; `bound`: columns that the common pages may
-    come to fill (0: as they are), of which `splits` is a function.  The quantum with the least estimated time: blocks run
-    on sms * PER_SM places, a page takes a block PAGE_US unless all together ask more of the memory than HBM_GBS."""
-    size = 2 if dtype == torch.bfloat16 else 4
-    common, own = [], []
+def shared_plan(lens: Tuple[int, ...], shared: Tuple[int, ...], group_rows: int, nkv: int, group: int, window: int,
+                dtype: torch.dtype, blocks: int, bound: int = 0) -> Tuple[int, int]:
+    """(row_blocks, parts): units that the rows of a group are split into, and the pieces of a unit that there is room for.  The
+    kernel cuts the line of all units' tiles into equal stretches, one per block; `parts` is what the longest unit then falls into with
+    two to spare (were there less room, the kernel would make the stretches longer).  `lens` and `shared` per group; `bound`: columns that
+    the common pages may come to fill while a recorded call is replayed."""
+    row_blocks = -(-group_rows // (BLOCK_ROWS[dtype] // group))
+    beams = -(-group_rows // row_blocks)
+    tile = TILE_PAGES[dtype]
+    total, longest = 0, 1
     for n, c in zip(lens, shared):
         first = max(0, n - window) // PAGE if window else 0
         end = -(-n // PAGE)
         border = min(max(c, first), end)
-        common.append(border - first)
-        own.append(end - border)
-    row_blocks = -(-group_rows // (BLOCK_ROWS // group))
-    page_us = PAGE_US[dtype] * head_dim / 128
-    places = sms * PER_SM[dtype]
-    pages = nkv * (sum(common) * row_blocks + sum(own) * group_rows)
-    floor = nkv * (sum(common) + sum(own) * group_rows) * PAGE * head_dim * 2 * size / (HBM_GBS * 1e3)
-    longest, most = max(common), max(own)
-    widest = max(longest, most, 1)
-    best = None
-    for q in [k for k in (1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 64, 96, 128, 192, 256) if k < widest] + [widest]:
-        tails = max(1, -(-most // q))
-        splits = max(1, -(-max(longest, bound) // q))
-        if splits + tails > MAX_PARTS:
-            continue
-        blocks = nkv * (sum(-(-c // q) for c in common) * row_blocks + sum(min(o, tails) for o in own) * group_rows)
-        work = pages * page_us + blocks * SETUP_US
-        t = max(floor + SETUP_US, work / places + 0.5 * (min(q, widest) * page_us + SETUP_US), min(q, widest) * page_us + SETUP_US)
-        t += MERGE_US + PART_US * (splits + tails)
-        if best is None or t < 0.99 * best[0]:
-            best = (t, splits, q, tails)
-    if best is None:             # very long: as many parts as the merge takes
-        tails = max(1, min(MAX_PARTS // 2, -(-most // 256)))
-        splits = MAX_PARTS - tails
-        return splits, max(1, -(-max(longest, bound) // splits)), tails
-    return best[1:]
+        tiles = -(-(border - first + (end - border) * beams) // tile)
+        total += tiles * row_blocks * nkv
+        longest = max(longest, tiles, -(-(max(bound, border - first) + (end - border) * beams) // tile) if bound else 0)
+    share = max(1, -(-total // blocks))
+    return row_blocks, max(2, min(MAX_PARTS, -(-longest // share) + 3))
 
 
 class SharedAttention:
@@ -77,7 +53,7 @@ class SharedAttention:
     def get(cls, dtype: torch.dtype, head_dim: int) -> Optional["SharedAttention"]:
         """The kernels for this type and head size, or None where there are none (the per-row kernels then read the same
         pages through the same tables)."""
-        if dtype not in MAX_GROUP or head_dim not in HEAD_DIMS:
+        if dtype not in MAX_HEADS or head_dim not in HEAD_DIMS:
             return None
         key = (dtype, head_dim)
         if key not in cls._known:
@@ -90,7 +66,7 @@ class SharedAttention:
 
     def _load(self) -> None:
         P, I, L = c_void_p, c_int, c_longlong
-        head = [P, P, P, L, P, P, P, P, P, I, P, P, I, I, I, I, I]
+        head = [P, P, P, L, P, P, P, P, P, P, I, P, P, I, I, I, I, I]
         rest = [I, c_float, I, I, I, P]
         if self.dtype == torch.bfloat16:
             name = f"attn_shared_bf16_hd{self.head_dim}"
@@ -107,7 +83,7 @@ class SharedAttention:
         self._call = call        # last: another thread calls as soon as it is there
 
     def takes(self, nh: int, nkv: int) -> bool:
-        return nkv > 0 and nh % nkv == 0 and nh // nkv <= MAX_GROUP[self.dtype]
+        return nkv > 0 and nh % nkv == 0 and nh // nkv <= MAX_HEADS[self.dtype]
 
     def decode(self, q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, out: torch.Tensor, seq_len: torch.Tensor,
                seq_slot: torch.Tensor, page_table: torch.Tensor, group_start: torch.Tensor, group_pages: torch.Tensor, nh: int,
@@ -143,21 +119,23 @@ class SharedAttention:
                 raise KernelError(f"shared attention: {n} lie on {t.device}, q on {q.device}")
         if rows == 0:
             return
-        if len(shared) != groups or groups == 0 or not 1 <= group_rows <= rows:
-            raise KernelError("shared attention: one length and one number of common pages per group are needed")
+        if len(shared) != groups or not 1 <= groups <= MAX_GROUPS or not 1 <= group_rows <= rows:
+            raise KernelError(f"shared attention: one length and one number of common pages per group are needed, at most {MAX_GROUPS} "
+                              "groups of at least one row")
         if min(lens) < 0 or max(lens) > page_table.shape[1] * PAGE or min(shared) < 0:
             raise KernelError(f"shared attention: lengths must lie in 0 to {page_table.shape[1] * PAGE}, numbers of pages be positive")
         if window is not None and window < 1:
             raise KernelError(f"shared attention: a window of {window}")
         if self._call is None:
             self._load()
-        splits, quantum, tails = shared_plan(tuple(lens), tuple(shared), group_rows, nkv, nh // nkv, hd, window or 0, self.dtype,
-                                             _sm_count(q.device), bound)
-        part = workspace.get("attn_shared_part", (rows * nh * (splits + tails) * (hd + 2),), torch.float32)
-        head = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, out.data_ptr(), part.data_ptr(), seq_len.data_ptr(),
-                seq_slot.data_ptr(), page_table.data_ptr(), page_table.stride(0), group_start.data_ptr(), group_pages.data_ptr(),
-                groups, rows, group_rows, nh, nkv)
-        rest = (window or 0, scale, splits, quantum, tails, _stream())
+        blocks = _sm_count(q.device)
+        row_blocks, parts = shared_plan(tuple(lens), tuple(shared), group_rows, nkv, nh // nkv, window or 0, self.dtype, blocks, bound)
+        part = workspace.get("attn_shared_part", (rows * nh * parts * (hd + 2),), torch.float32)
+        pieces = workspace.get("attn_shared_pieces", (groups * row_blocks * nkv,), torch.int32)
+        head = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, out.data_ptr(), part.data_ptr(), pieces.data_ptr(),
+                seq_len.data_ptr(), seq_slot.data_ptr(), page_table.data_ptr(), page_table.stride(0), group_start.data_ptr(),
+                group_pages.data_ptr(), groups, rows, group_rows, nh, nkv)
+        rest = (window or 0, scale, row_blocks, parts, blocks, _stream())
         _check(self._call(*head, *rest) if self.dtype == torch.bfloat16 else self._call(*head, hd, *rest), "attn_shared")
         _check(0, "attn_shared_merge")
 
@@ -169,6 +147,8 @@ def run_shared(q, cache_view, out, batch, nh: int, nkv: int, window, scale: floa
     if kernel is None or not kernel.takes(nh, nkv):
         return False
     g, c = batch.groups, cache_view
+    if len(g.rows) > MAX_GROUPS:
+        return False
     seen = min(batch.len_bucket, window + PAGE) if window else batch.len_bucket
     kernel.decode(q, c.k_pages, c.v_pages, out, batch.seq_len, batch.seq_slot, c.page_table, g.start, g.pages, nh, nkv, window, scale,
                   workspace, lens=g.lens, shared=g.shared, group_rows=max(g.rows), bound=-(-seen // PAGE))
