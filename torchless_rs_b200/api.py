@@ -119,7 +119,7 @@ class Model:
 
         def select(logits, scores, n):
             on_device = torch.tensor(scores, dtype=torch.float32).to(logits.device)
-            out = self.beam_selector.ops.select(logits, on_device, n).cpu()
+            out = self.beam_selector.ops.select(logits, on_device, n)[:3].cpu()
             return out[0].view(torch.float32), out[1], out[2]
 
         results = _generate_beams(self.engine, select, prompts, max_tokens, beams, length_penalty, stop_ids, n_best, early_stop,

@@ -17,8 +17,8 @@
 // from the keys that the row sees alone.
 //
 // The tiles of all units lie in one line, which the blocks (one per SM) cut into equal stretches: nobody waits for the longest
-// sequence, and loads run on across units.  A unit that lies in one stretch is written to `out`; pieces leave a maximum, a sum and a weighted
-// sum per row and head, and a second kernel merges them in the order of the keys.  What bounds this is the memory: a tile of head
+// sequence, and loads run on across units.  A stretch of a unit leaves a reference, a sum and a
+// weighted sum per row and head, and a second kernel merges them in the order of the keys.  What bounds this is the memory: a tile of head
 // size 128 is 64 KB and takes an SM 1.5 us at the copy rate; its softmax and products take about a third of that.
 //
 // Nothing is read before the wait for the kernels before: a page may have been copied by one of them.  Every wait on an mbarrier
@@ -320,6 +320,8 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       const int upper = warp >> 2, key = tid & 127, page_of = key >> 6, first_col = upper * NC, quad = warp & 3;
       const uint32_t t_lane = (uint32_t)(quad * 32) << 16;
       volatile int* moved = moved_s + 3 * upper;
+      const int my_col = first_col + (key & (NC - 1)), my_beam = my_col / G, my_head = my_col - my_beam * G;
+      const int first_beam = first_col / G, first_head = first_col - first_beam * G;
       auto load_q = [&](const ShPiece& p, int buf) {
         uint8_t* dst = q_s + buf * Z::Q;
         for (int i = tid; i < N * (HEAD_DIM / 8); i += SH_SOFT) {
@@ -346,10 +348,6 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         const int last = min(p.tiles, p.tile + t1 - t), R = p.beams * G;
         const int next = t + last - p.tile;
         ShPiece np = p;
-        if (next < t1) {                       // the next unit's queries: its buffer's scores were all read a unit ago
-          np = sh_locate<2>(table, a, next);
-          load_q(np, (unit + 1) & 1);
-        }
 #pragma unroll
         for (int c = 0; c < NC; ++c) l[c] = neg_ref[c] = 0.0f;
         if (key < NC) {
@@ -459,6 +457,11 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           sh_async_fence();
           tc_fence_before();
           sh_arrive(&p_full[buf]);
+          if (j == p.tile && next < t1) {
+            // the next unit's queries: its buffer's scores were all read a unit ago
+            np = sh_locate<2>(table, a, next);
+            load_q(np, (unit + 1) & 1);
+          }
           // two pages on
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -479,36 +482,27 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         const int slot = (int)blockIdx.x - first_block;
         if (tid == 0 && slot == 0) a.unit_parts[p.unit] = pieces;
         // (What runs once per unit is fetched from afar, some ten cycles an instruction: it is written as loops, without divisions.)
-        const int my_r = first_col + key;
-        if (key < NC && my_r < R) {
-          const float sum = (red_s[my_r] + red_s[N + my_r]) + (red_s[2 * N + my_r] + red_s[3 * N + my_r]);
-          al_s[my_r] = pieces > 1 ? 1.0f : 1.0f / sum;
-          if (pieces > 1) {
-            const int beam = my_r / G;
-            float* dst = a.part + (((size_t)(p.row0 + beam) * a.nh + p.kvh * G + my_r - beam * G) * a.parts + slot) * SH_STRIDE + HEAD_DIM;
-            dst[0] = ref_s[my_r];
-            dst[1] = sum;
-          }
+        const int heads = a.parts * SH_STRIDE;
+        if (key < NC && my_col < R) {
+          float* dst = a.part + ((size_t)(p.row0 + my_beam) * a.nh + p.kvh * G + my_head) * heads + slot * SH_STRIDE + HEAD_DIM;
+          dst[0] = ref_s[my_col];
+          dst[1] = (red_s[my_col] + red_s[N + my_col]) + (red_s[2 * N + my_col] + red_s[3 * N + my_col]);
         }
-        sh_bar(upper);
         sh_park(&pv_done[(n - 1) & 1], (uint32_t)((n - 1) >> 1) & 1u, abort_flag, 13);
         tc_fence_after();
         if (key < HEAD_DIM) {                  // (whole warps)
-          int beam = first_col / G, g = first_col - beam * G;
-          size_t head = (size_t)(p.row0 + beam) * a.nh + p.kvh * G + g;
+          float* dst = a.part + ((size_t)(p.row0 + first_beam) * a.nh + p.kvh * G + first_head) * heads + slot * SH_STRIDE + key;
+          int left = G - first_head;           // heads to the end of the beam
+          const int n_col = min(R - first_col, NC);
 #pragma unroll 1
-          for (int c = 0; c < NC && first_col + c < R; c += 8) {
+          for (int c = 0; c < n_col; c += 8) {
             float o[8];
             sh_tmem_ld<8>(tmem_o + t_lane + first_col + c, o);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const int r = first_col + c + e;
-              if (r < R) {
-                if (pieces > 1) a.part[(head * a.parts + slot) * SH_STRIDE + key] = o[e];
-                else a.out[head * HEAD_DIM + key] = __float2bfloat16_rn(o[e] * al_s[r]);
-              }
-              ++head;
-              if (++g == G) { g = 0; head += a.nh - G; }
+              if (c + e < n_col) *dst = o[e];
+              dst += heads;
+              if (--left == 0) { left = G; dst += (size_t)(a.nh - G) * heads; }
             }
           }
         }

@@ -141,8 +141,7 @@ __device__ __forceinline__ void sh_page(const ShPiece& p, int i, int& owner, int
   }
 }
 
-// Merges the pieces of one (row, head), a thread per dimension, in the order of the keys; a unit in one piece has been
-// written.  A row without any key (of length 0) gives zero.  EXP2: the maxima are logarithms to the base 2.
+// Merges the pieces of one (row, head), a thread per dimension, in the order of the keys.  A row without any key (of length 0) gives zero.  EXP2: the maxima are logarithms to the base 2.
 //
 // AGAIN: a result that is no number is computed again from the keys that the row sees, one page after the other (the first kernel
 // multiplies values that it does not see by zero).  That is slow, and needed only where the cache holds values that are no numbers.
@@ -172,41 +171,39 @@ attn_shared_merge_kernel(const ShArgs<T> a, const T* __restrict__ k_pages, const
 #pragma unroll
   for (int s = 0; s < AHEAD; ++s) v[s] = s < a.parts ? src[s * (HD + 2) + d] : 0.0f;
   const int kvh = h / (a.nh / a.nkv), parts = a.unit_parts[((size_t)g * a.row_blocks + in_group / a.beams) * a.nkv + kvh];
-  float result;
-  if (parts <= 1) {
-    if (!AGAIN) return;
-    result = to_f32(a.out[head * HD + d]);
-  } else {
-    // every warp: the largest reference, the factors, the sum (a piece in which this row sees no key has a reference of -inf)
-    constexpr int ROUNDS = (SH_MAX_PARTS + 31) / 32;
-    float ref[ROUNDS], sum[ROUNDS], m = -INFINITY, l = 0.0f;
+  // every warp: the largest reference, the factors, the sum (a piece in which this row sees no key has a reference of -inf)
+  constexpr int ROUNDS = (SH_MAX_PARTS + 31) / 32;
+  float ref[ROUNDS], sum[ROUNDS], m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < ROUNDS; ++i) {
-      const int s = lane + 32 * i;
-      ref[i] = s < parts ? src[s * (HD + 2) + HD] : -INFINITY;
-      sum[i] = s < parts ? src[s * (HD + 2) + HD + 1] : 0.0f;
-      m = fmaxf(m, ref[i]);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-#pragma unroll
-    for (int i = 0; i < ROUNDS; ++i) {
-      const float f = ref[i] == -INFINITY ? 0.0f : EXP2 ? exp2f(ref[i] - m) : expf(ref[i] - m);
-      l += f * sum[i];
-      if (d < 32 && lane + 32 * i < SH_MAX_PARTS) f_s[lane + 32 * i] = f;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    __syncthreads();
-    float acc = 0.0f;
-#pragma unroll
-    for (int s = 0; s < AHEAD; ++s)
-      if (s < parts) acc += f_s[s] * v[s];
-#pragma unroll 8
-    for (int s = AHEAD; s < parts; ++s) acc += f_s[s] * src[s * (HD + 2) + d];
-    result = acc / l;
-    store(result);
+  for (int i = 0; i < ROUNDS; ++i) {
+    ref[i] = -INFINITY;
+    sum[i] = 0.0f;
+    if (32 * i >= parts) continue;       // (few pieces: little of this is fetched and run)
+    const int s = lane + 32 * i;
+    ref[i] = s < parts ? src[s * (HD + 2) + HD] : -INFINITY;
+    sum[i] = s < parts ? src[s * (HD + 2) + HD + 1] : 0.0f;
+    m = fmaxf(m, ref[i]);
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    if (32 * i >= parts) break;
+    const float f = ref[i] == -INFINITY ? 0.0f : EXP2 ? exp2f(ref[i] - m) : expf(ref[i] - m);
+    l += f * sum[i];
+    if (d < 32 && lane + 32 * i < SH_MAX_PARTS) f_s[lane + 32 * i] = f;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  __syncthreads();
+  float acc = 0.0f;
+#pragma unroll
+  for (int s = 0; s < AHEAD; ++s)
+    if (s < parts) acc += f_s[s] * v[s];
+#pragma unroll 8
+  for (int s = AHEAD; s < parts; ++s) acc += f_s[s] * src[s * (HD + 2) + d];
+  const float result = acc / l;
+  store(result);
   if constexpr (AGAIN) {
     if (!__syncthreads_or(!isfinite(result))) return;
     __shared__ float p_s[PAGE];

@@ -9,7 +9,7 @@ from typing import Dict, Optional, Sequence, Tuple
 import torch
 
 from . import build
-from .ops import KernelError, _check, _here, _need, _sm_count, _stream, register_error_word
+from .ops import KernelError, _check, _here, _stream_on, register_error_word
 
 HEAD_DIMS = (64, 128)
 PAGE = build.PAGE_TOKENS
@@ -44,6 +44,15 @@ def shared_plan(lens: Tuple[int, ...], shared: Tuple[int, ...], group_rows: int,
         longest = max(longest, tiles, -(-(max(bound, border - first) + (end - border) * beams) // tile) if bound else 0)
     share = max(1, -(-total // blocks))
     return row_blocks, max(2, min(MAX_PARTS, -(-longest // share) + 3))
+
+
+_sms: Dict[int, int] = {}
+
+
+def _sm_count(device: int) -> int:
+    if device not in _sms:
+        _sms[device] = torch.cuda.get_device_properties(device).multi_processor_count
+    return _sms[device]
 
 
 class SharedAttention:
@@ -98,25 +107,21 @@ class SharedAttention:
         hd, rows, groups = self.head_dim, q.shape[0], len(lens)
         if not self.takes(nh, nkv):
             raise KernelError(f"shared attention: {nh} query heads over {nkv} are not taken")
-        _here(q, "shared attention q")
-        for t, n in ((q, "q"), (k_pages, "k pages"), (v_pages, "v pages"), (out, "out")):
-            _need(t, self.dtype, f"shared attention {n}")
+        dev = _here(q, "shared attention q")
         pages = k_pages.shape[0]
         if q.shape != (rows, nh * hd) or out.shape != q.shape or k_pages.shape != (pages, nkv, PAGE, hd) or \
                 v_pages.shape != (pages, nkv, hd, PAGE):
             raise KernelError(f"shared attention: shapes do not fit: q {tuple(q.shape)}, out {tuple(out.shape)}, k pages "
                               f"{tuple(k_pages.shape)}, v pages {tuple(v_pages.shape)}, {nh} heads over {nkv} of {hd}")
-        for t, n, count in ((seq_len, "lengths", rows), (seq_slot, "slots", rows), (group_start, "group starts", groups + 1),
-                            (group_pages, "group pages", groups)):
-            _need(t, torch.int32, f"shared attention {n}")
-            if t.numel() != count:
-                raise KernelError(f"shared attention: {count} {n} are needed, got {t.numel()}")
-        if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1:
-            raise KernelError("shared attention: the page table must be int32 [slots, columns]")
-        for t, n in ((k_pages, "k pages"), (v_pages, "v pages"), (out, "out"), (seq_len, "lengths"), (seq_slot, "slots"),
-                     (page_table, "page table"), (group_start, "group starts"), (group_pages, "group pages")):
-            if t.device != q.device:
-                raise KernelError(f"shared attention: {n} lie on {t.device}, q on {q.device}")
+        for t in (q, k_pages, v_pages, out):
+            if t.dtype != self.dtype or not t.is_contiguous() or t.get_device() != dev:
+                raise KernelError(f"shared attention: q, out, k pages and v pages must be contiguous {self.dtype} tensors on one device")
+        for t, count in ((seq_len, rows), (seq_slot, rows), (group_start, groups + 1), (group_pages, groups)):
+            if t.dtype != torch.int32 or t.numel() != count or not t.is_contiguous() or t.get_device() != dev:
+                raise KernelError(f"shared attention: {rows} lengths and slots, {groups + 1} group starts and {groups} group pages are "
+                                  f"needed, contiguous int32 on {q.device}")
+        if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1 or page_table.get_device() != dev:
+            raise KernelError(f"shared attention: the page table must be int32 [slots, columns] on {q.device}")
         if rows == 0:
             return
         if len(shared) != groups or not 1 <= groups <= MAX_GROUPS or not 1 <= group_rows <= rows:
@@ -128,14 +133,14 @@ class SharedAttention:
             raise KernelError(f"shared attention: a window of {window}")
         if self._call is None:
             self._load()
-        blocks = _sm_count(q.device)
+        blocks = _sm_count(dev)
         row_blocks, parts = shared_plan(tuple(lens), tuple(shared), group_rows, nkv, nh // nkv, window or 0, self.dtype, blocks, bound)
         part = workspace.get("attn_shared_part", (rows * nh * parts * (hd + 2),), torch.float32)
         pieces = workspace.get("attn_shared_pieces", (groups * row_blocks * nkv,), torch.int32)
         head = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, out.data_ptr(), part.data_ptr(), pieces.data_ptr(),
                 seq_len.data_ptr(), seq_slot.data_ptr(), page_table.data_ptr(), page_table.stride(0), group_start.data_ptr(),
                 group_pages.data_ptr(), groups, rows, group_rows, nh, nkv)
-        rest = (window or 0, scale, row_blocks, parts, blocks, _stream())
+        rest = (window or 0, scale, row_blocks, parts, blocks, _stream_on(dev))
         _check(self._call(*head, *rest) if self.dtype == torch.bfloat16 else self._call(*head, hd, *rest), "attn_shared")
         _check(0, "attn_shared_merge")
 

@@ -262,8 +262,7 @@ attn_shared_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 #pragma unroll
     for (int d = TR / 2; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
     auto head_of = [&](int r) { return (size_t)(p.row0 + r / G) * a.nh + p.kvh * G + r % G; };
-    if (sk == 0) al_s[sr] = l;
-    if (sk == 0 && sr < R && pieces > 1) {
+    if (sk == 0 && sr < R) {
       float* dst = a.part + (head_of(sr) * a.parts + slot) * (HD + 2) + HD;
       dst[0] = m;
       dst[1] = l;
@@ -286,9 +285,7 @@ attn_shared_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       float o = 0.0f;
 #pragma unroll
       for (int k = 0; k < KV / HALVES; ++k) o += o_s[k * ROWS * HD + i];
-      const int r = i / HD, d = i % HD;
-      if (pieces > 1) a.part[(head_of(r) * a.parts + slot) * (HD + 2) + d] = o;
-      else a.out[head_of(r) * HD + d] = o / al_s[r];
+      a.part[(head_of(i / HD) * a.parts + slot) * (HD + 2) + i % HD] = o;
     }
     t = next;
     p = np;

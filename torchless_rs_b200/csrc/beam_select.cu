@@ -4,16 +4,18 @@
 //
 //   v(b, t) = c_b + x_bt - log sum_u exp x_bu        the n largest of all (b, t) in falling order; ties: lowest (b, t) first
 //
-// Two kernels.  The first reads every row once: a block holds a part of a row in registers, takes its maximum M and the
-// sum of exp(x - M), and keeps its n largest entries.  Within a row the constant c_b - lse does not matter, so a part's n
-// largest x are all that can become a candidate.  Which those are: the threads form groups, and the n-th largest of the
-// groups' maxima is a bound that at least n entries reach; few others do (22 for n = 16), those go to shared memory and are
-// ranked by counting.  The second kernel, a block per sequence, joins the parts of each row and takes the n
-// largest of the parts' candidates the same way.
+// Two kernels.  The first reads every row once, a block per part of a row.  Within a row the constant c_b - lse does not matter, so
+// a part's n largest x are all that can become a candidate.  An entry that reaches a bound that n entries are known to reach is
+// collected in shared memory, any other is added to the sum of exp(x - bound), in which nothing can overflow.  The first bound comes of
+// the part's first 4096 entries (the threads form groups, and the n-th largest of the groups' maxima is reached by n entries and, for n = 16,
+// by 22 in all); whenever the tiles read have doubled, the n-th largest of those collected becomes the next, so that ever fewer
+// are collected (some 20 in each doubling) and the threads hardly ever wait for each other.  In the end the collected entries are added
+// in 64 bits and ranked by counting.  The second kernel, a block per sequence, joins the parts of each row and takes the n
+// largest of their candidates the same way.
 //
 // Candidates of different beams are compared by sums of 32-bit numbers whose logarithm is rounded too, so which comes first is decided
-// in 64 bits: exp runs in 32 bits, but its results are added without rounding (below), the parts' sums are joined in 64 bits, and the
-// entries with weight (each part's n largest) are then exchanged for their exp in 64 bits.
+// in 64 bits: the entries with weight are those that are collected; the exp of the others runs in 32 bits, and their results are added
+// without rounding (below).
 //
 // An entry that is NaN counts as -inf, +inf as the largest finite number; an entry of -inf is no candidate.
 #include <cuda_runtime.h>
@@ -39,24 +41,59 @@ __device__ __forceinline__ float bs_value(uint32_t k) {
 }
 // a number that does not order as one (NaN) as -inf, +inf as the largest finite one
 __device__ __forceinline__ float bs_clean(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }
-__device__ __forceinline__ float bs_exp(float x, float m) {   // 0 for x = -inf; m is finite
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((x - m) * LOG2E));
-  return e;
+// two 32-bit numbers in one register pair, and sm_100's arithmetic on them
+__device__ __forceinline__ u64 bs_pair(float a, float b) {
+  u64 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void bs_unpair(u64 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ u64 bs_add2(u64 a, u64 b) {
+  u64 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ u64 bs_mul2(u64 a, u64 b) {
+  u64 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ u64 bs_fma2(u64 a, u64 b, u64 c) {
+  u64 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ float bs_max3(float a, float b, float c) {     // (passes over NaN)
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
 }
 __device__ __forceinline__ u64 max_u64(u64 a, u64 b) { return a > b ? a : b; }
+__device__ __forceinline__ u64 bs_warp_max(u64 w) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) w = max_u64(w, __shfl_xor_sync(0xffffffffu, w, o));
+  return w;
+}
 
-// What the first kernel leaves for the second, per (row, part): the part's maximum and sum, how many candidates follow.
+// What the first kernel leaves for the second, per (row, part): the largest entry M, the sum of exp(x - M), how many candidates follow.
 struct BsPart {
   double sum;
   float max;
   int count;
 };
 
-// E entries per thread; GS threads form a group (256 / GS >= 2 n groups, or as many as there are threads).
-template <int E, int GS>
-__global__ void __launch_bounds__(BS_THREADS)
-beam_rows_kernel(const float* __restrict__ logits, long long ld, int V, const float* __restrict__ scores, int n, int parts,
+#define BS_TILE (BS_THREADS * 16)
+#ifndef BS_MAX_TILES
+#define BS_MAX_TILES 32
+#endif
+#ifndef BS_PER_SM
+#define BS_PER_SM 4                // resident blocks
+#endif
+
+// GS threads form a group (256 / GS >= 2 n groups, or as many as there are threads).
+template <int GS>
+__global__ void __launch_bounds__(BS_THREADS, BS_PER_SM)
+beam_rows_kernel(const float* __restrict__ logits, long long ld, int V, const float* __restrict__ scores, int n, int chunk,
                  BsPart* __restrict__ part, uint2* __restrict__ cand) {
   constexpr int GROUPS = BS_THREADS / GS;
   __shared__ u64 gm[GROUPS];
@@ -68,7 +105,7 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, int V, const fl
   pdl_wait();
   pdl_launch_dependents();
   const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const size_t slot = (size_t)row * parts + blockIdx.x;
+  const size_t slot = (size_t)row * gridDim.x + blockIdx.x;
   const float score = scores[row];
   if (!(score > -INFINITY)) {     // no beam: its row is not read
     if (tid == 0) part[slot] = {0.0, -INFINITY, 0};
@@ -77,116 +114,219 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, int V, const fl
   // The entries in fours on 16-byte boundaries of memory: `shift` entries before the row's first belong to the row before.
   const float* x0 = logits + (size_t)row * ld;
   const int shift = (int)(((uintptr_t)x0 >> 2) & 3);
-  const int first = blockIdx.x * (BS_THREADS * E) - shift;
-  float x[E];
+  const int first = blockIdx.x * chunk - shift, end = min(first + chunk, V);
+  // Entry j of this thread in the tile that begins at i0.
+  auto index = [&](int i0, int j) { return i0 + ((j >> 2) * BS_THREADS + tid) * 4 + (j & 3); };
+  const float* mine0 = x0 + first + tid * 4;
+  bool nans = false;              // entries that are NaN were met: they become -inf as they are loaded
+  auto load = [&](int i0, float (&x)[16]) {
+    if (i0 >= 0 && i0 + BS_TILE <= end) {              // (a whole tile)
+      const float* p = mine0 + (i0 - first);
 #pragma unroll
-  for (int k = 0; k < E / 4; ++k) {
-    const int i = first + (k * BS_THREADS + tid) * 4;
-    if (i >= 0 && i + 3 < V) {
-      const float4 v = __ldcs(reinterpret_cast<const float4*>(x0 + i));
-      x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
+      for (int k = 0; k < 4; ++k) {
+        const float4 v = __ldcs(reinterpret_cast<const float4*>(p + k * BS_THREADS * 4));
+        x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * k + e] = i + e >= 0 && i + e < V ? x0[i + e] : -INFINITY;
+      for (int j = 0; j < 16; ++j) {
+        const int i = index(i0, j);
+        x[j] = i >= 0 && i < end ? x0[i] : -INFINITY;
+      }
     }
-  }
-  // entry number k * 4 + e of this thread; a word orders entries by value, equal ones by index, lowest first
-  auto index = [&](int j) { return first + ((j >> 2) * BS_THREADS + tid) * 4 + (j & 3); };
-  auto word = [&](int j) { return ((u64)bs_key(x[j]) << 32) | (uint32_t)~index(j); };
-  float best = -INFINITY;
-  int best_j = 0;
+    if (nans) {
 #pragma unroll
-  for (int j = 0; j < E; ++j) {
-    x[j] = bs_clean(x[j]);
-    if (x[j] > best) { best = x[j]; best_j = j; }
-  }
-  u64 w = ((u64)bs_key(best) << 32) | (uint32_t)~index(best_j);
+      for (int j = 0; j < 16; ++j) x[j] = fmaxf(x[j], -INFINITY);
+    }
+  };
+  // A word orders entries by value, equal ones by index, lowest first.
+  auto word = [&](float x, int i) { return ((u64)bs_key(x) << 32) | (uint32_t)~i; };
+
+  float x[16];
+  load(first, x);
+  {
+    float best = -INFINITY;
+    int best_j = 0;
 #pragma unroll
-  for (int o = 1; o < GS; o <<= 1) w = max_u64(w, __shfl_xor_sync(0xffffffffu, w, o));
-  if (tid % GS == 0) gm[tid / GS] = w;
+    for (int j = 0; j < 16; ++j)
+      if (x[j] > best) { best = x[j]; best_j = j; }
+    u64 w = best > -INFINITY ? word(fminf(best, FLT_MAX), index(first, best_j)) : 0;
+#pragma unroll
+    for (int o = 1; o < GS; o <<= 1) w = max_u64(w, __shfl_xor_sync(0xffffffffu, w, o));
+    if (tid % GS == 0) gm[tid / GS] = w;
+  }
   if (tid == 0) count = 0;
   __syncthreads();
-  // the block's maximum, in every warp
-  u64 top = 0;
-#pragma unroll
-  for (int k = 0; k < GROUPS; k += 32) top = max_u64(top, gm[k + lane]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max_u64(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float M = bs_value((uint32_t)(top >> 32));
-  if (M == -INFINITY) {           // nothing here can follow (the same in all threads)
-    if (tid == 0) part[slot] = {0.0, -INFINITY, 0};
-    return;
-  }
-  if (tid < GROUPS) {             // the n-th largest of the groups' maxima (they all differ: an index is part of each)
+  if (tid < GROUPS) {             // the n-th largest of the groups' maxima (but for empty groups they all differ: an index is part of each)
     const u64 mine = gm[tid];
     int rank = 0;
 #pragma unroll 8
-    for (int k = 0; k < GROUPS; ++k) rank += gm[k] > mine ? 1 : 0;
+    for (int k = 0; k < GROUPS; ++k) rank += gm[k] > mine || (gm[k] == mine && k < tid) ? 1 : 0;
     if (rank == (n < GROUPS ? n : GROUPS) - 1) bound = mine;
   }
+  __syncthreads();
+
   // Each exp lies in [0, 1]; 1536 has a last place of 2^-13, so (e + 1536) - 1536 is e's part above that and what is left is exact too.
-  // Up to 32 upper parts add without rounding, and the lower ones' roundings are below 2^-37.
-  float hi = 0.0f, lo = 0.0f;
+  // The upper parts of up to 2048 entries add without rounding, and the lower ones' roundings are below 2^-34.  (Another bound
+  // scales both sums, which rounds a thread's share of them by 2^-24.)
+  float ref = 0.0f, bv;
+  u64 b, hi, lo;                  // (sums of two kinds of places)
+  const u64 log2e = bs_pair(LOG2E, LOG2E), up = bs_pair(1536.0f, 1536.0f), down = bs_pair(-1536.0f, -1536.0f), minus = bs_pair(-1.0f, -1.0f);
+  auto take_bound = [&] {         // 0: fewer than n entries so far, all of which are collected
+    b = bound;
+    const float now = b ? bs_value((uint32_t)(b >> 32)) : 0.0f;
+    bv = b ? now : -INFINITY;
+    float f;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(fminf((ref - now) * LOG2E, 0.0f)));
+    hi = bs_mul2(hi, bs_pair(f, f));
+    lo = bs_mul2(lo, bs_pair(f, f));
+    ref = now;
+  };
+  auto take = [&](int i0, float (&v)[16]) {
+    const u64 neg_ref = bs_pair(-ref, -ref);
 #pragma unroll
-  for (int j = 0; j < E; ++j) {
-    const float e = bs_exp(x[j], M);
-    const float h = __fsub_rn(__fadd_rn(e, 1536.0f), 1536.0f);
-    hi += h;
-    lo += e - h;
+    for (int k = 0; k < 16; k += 8) {
+      const float m8 = bs_max3(bs_max3(v[k], v[k + 1], v[k + 2]), bs_max3(v[k + 3], v[k + 4], v[k + 5]), fmaxf(v[k + 6], v[k + 7]));
+      if (__any_sync(0xffffffffu, m8 >= bv)) {       // (a vote, so that this is a branch)
+#pragma unroll
+        for (int e = k; e < k + 8; ++e) {
+          if (v[e] >= bv && v[e] > -INFINITY) {
+            const u64 w = word(fminf(v[e], FLT_MAX), index(i0, e));
+            if (w >= b) {
+              const int at = atomicAdd(&count, 1);
+              if (at < BS_CAP) buf[at] = w;
+              v[e] = -INFINITY;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int e = k; e < k + 8; e += 2) {
+        float p0, p1;
+        bs_unpair(bs_mul2(bs_add2(bs_pair(v[e], v[e + 1]), neg_ref), log2e), p0, p1);
+        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(p0));
+        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(p1));
+        const u64 p = bs_pair(p0, p1), h = bs_add2(bs_add2(p, up), down);
+        hi = bs_add2(hi, h);
+        lo = bs_add2(lo, bs_fma2(h, minus, p));
+      }
+    }
+  };
+  hi = lo = bs_pair(0.0f, 0.0f);
+  take_bound();
+  for (;;) {
+    int next = first + BS_TILE;   // where the bound is looked at again: after 1, 2, 4, ... tiles
+    auto look = [&](int i0) {
+      if (i0 != next || next >= end) return;
+      next = first + 2 * (next - first);
+      __syncthreads();
+      const int c = min(count, BS_CAP);
+      for (int i = tid; i < c; i += BS_THREADS) {
+        const u64 mine = buf[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int k = 0; k < c; ++k) rank += buf[k] > mine ? 1 : 0;
+        if (rank == n - 1) bound = mine;
+      }
+      __syncthreads();
+      take_bound();
+    };
+#pragma unroll 1
+    for (int i0 = first; i0 < end; i0 += 2 * BS_TILE) {
+      float y[16];
+      if (i0 + BS_TILE < end) load(i0 + BS_TILE, y);           // the next tile is on its way while one is summed
+      take(i0, x);
+      look(i0 + BS_TILE);
+      if (i0 + BS_TILE >= end) break;
+      if (i0 + 2 * BS_TILE < end) load(i0 + 2 * BS_TILE, x);
+      take(i0 + BS_TILE, y);
+      look(i0 + 2 * BS_TILE);
+    }
+    // a NaN has come into a sum: once more without, and with the bound that has been found
+    float h0, h1;
+    bs_unpair(hi, h0, h1);
+    if (__syncthreads_or(!nans && h0 + h1 != h0 + h1)) {
+      nans = true;
+      if (tid == 0) count = 0;
+      hi = lo = bs_pair(0.0f, 0.0f);
+      load(first, x);
+      __syncthreads();
+      take_bound();
+      continue;
+    }
+    if (count <= BS_CAP) break;
+    // More entries were collected than there is room for (they rise along the row, or bunch in few groups): the n-th largest of
+    // the part, found one after the other, each the largest below the one before; then the same again with that as the bound.
+    u64 last = ~0ull;
+    for (int r = 0; r < n; ++r) {
+      u64 w = 0;
+#pragma unroll 1
+      for (int i = first + tid; i < end; i += BS_THREADS) {
+        const float v = i >= 0 ? bs_clean(x0[i]) : -INFINITY;
+        const u64 wi = word(v, i);
+        if (v > -INFINITY && wi < last) w = max_u64(w, wi);
+      }
+      w = bs_warp_max(w);
+      if (lane == 0) wmax[warp] = w;
+      __syncthreads();
+      for (int k = 0; k < BS_THREADS / 32; ++k) w = max_u64(w, wmax[k]);
+      __syncthreads();
+      last = w;                   // more than BS_CAP >= n entries are there, so w is one
+    }
+    if (tid == 0) { bound = last; count = 0; }
+    __syncthreads();
+    hi = lo = bs_pair(0.0f, 0.0f);
+    take_bound();
+    load(first, x);
   }
-  double sum = (double)hi + (double)lo;
+
+  // ---- the part's maximum, its sum, its n largest
+  const int c = count;
+  if (c == 0) {                   // nothing here can follow
+    if (tid == 0) part[slot] = {0.0, -INFINITY, 0};
+    return;
+  }
+  u64 w = 0;
+  for (int i = tid; i < c; i += BS_THREADS) w = max_u64(w, buf[i]);
+  w = bs_warp_max(w);
+  if (lane == 0) wmax[warp] = w;
+  __syncthreads();
+  const float M = bs_value((uint32_t)(bs_warp_max(wmax[lane & (BS_THREADS / 32 - 1)]) >> 32));
+  // the entries that were not collected, then the collected ones
+  double rest;
+  {
+    float h0, h1, l0, l1;
+    bs_unpair(hi, h0, h1);
+    bs_unpair(lo, l0, l1);
+    rest = ((double)h0 + (double)h1) + ((double)l0 + (double)l1);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
+  double sum = 0.0;
+  // (lane 0 of a warp has the warp's rest beside its entries)
+  for (int i = lane == 0 ? tid - BS_THREADS : tid; i < c; i += BS_THREADS) {
+    const double weight = i < 0 ? rest : 1.0;
+    const double at = i < 0 ? (double)ref : (double)bs_value((uint32_t)(buf[i] >> 32));
+    if (weight != 0.0) sum += weight * exp(at - (double)M);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) wsum[warp] = sum;
-  __syncthreads();
-  const u64 b = bound;
-  const float bv = bs_value((uint32_t)(b >> 32));
-#pragma unroll
-  for (int j = 0; j < E; ++j) {
-    if (x[j] >= bv && x[j] > -INFINITY) {
-      const u64 wj = word(j);
-      if (wj >= b) {
-        const int at = atomicAdd(&count, 1);
-        if (at < BS_CAP) buf[at] = wj;
-      }
-    }
-  }
-  __syncthreads();
-  const int c = count;
   uint2* out = cand + slot * n;
-  if (c <= BS_CAP) {
-    for (int i = tid; i < c; i += BS_THREADS) {
-      const u64 mine = buf[i];
-      int rank = 0;
-      for (int k = 0; k < c; ++k) rank += buf[k] > mine ? 1 : 0;
-      if (rank < n) out[rank] = make_uint2((uint32_t)(mine >> 32), ~(uint32_t)mine);
-    }
-  } else {
-    // entries bunch in fewer than n groups: one after the other, each the largest below the one before
-    u64 last = ~0ull;
-    for (int r = 0; r < n; ++r) {
-      u64 m = 0;
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const u64 wj = word(j);
-        if (x[j] > -INFINITY && wj < last) m = max_u64(m, wj);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = max_u64(m, __shfl_xor_sync(0xffffffffu, m, o));
-      if (lane == 0) wmax[warp] = m;
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < BS_THREADS / 32; ++k) m = max_u64(m, wmax[k]);
-      __syncthreads();
-      last = m;                   // more than BS_CAP >= n entries are there, so m is one
-      if (tid == 0) out[r] = make_uint2((uint32_t)(m >> 32), ~(uint32_t)m);
-    }
+  for (int i = tid; i < c; i += BS_THREADS) {
+    const u64 mine = buf[i];
+    if (mine < b) continue;       // (n entries reach the last bound)
+    int rank = 0;
+#pragma unroll 8
+    for (int k = 0; k < c; ++k) rank += buf[k] > mine ? 1 : 0;
+    if (rank < n) out[rank] = make_uint2((uint32_t)(mine >> 32), ~(uint32_t)mine);
   }
-  if (tid == 0) {
-    double s = 0.0;
+  __syncthreads();
+  if (warp == 0) {
+    sum = lane < BS_THREADS / 32 ? wsum[lane] : 0.0;
 #pragma unroll
-    for (int k = 0; k < BS_THREADS / 32; ++k) s += wsum[k];
-    part[slot] = {s, M, c < n ? c : n};
+    for (int o = BS_THREADS / 64; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) part[slot] = {sum, M, c < n ? c : n};
   }
 }
 
@@ -199,63 +339,79 @@ __device__ __forceinline__ BsCand bs_shfl(const BsCand& a, int o) {
   return {__shfl_xor_sync(0xffffffffu, a.v, o), __shfl_xor_sync(0xffffffffu, a.at, o)};
 }
 
-template <int GS>
+// CAND: candidates of a sequence per thread that are held in registers; 0: any number, read again for every look at them.
+template <int GS, int CAND>
 __global__ void __launch_bounds__(BS_THREADS)
 beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ cand, const float* __restrict__ scores, int B, int V,
                   int n, int parts, float* __restrict__ values, int* __restrict__ beams, int* __restrict__ tokens) {
-  constexpr int GROUPS = BS_THREADS / GS;
-  extern __shared__ double base[];        // [B]: c_b - lse_b
+  constexpr int GROUPS = BS_THREADS / GS, HELD = CAND ? CAND : 1;
+  extern __shared__ double lse[];         // [B]
   __shared__ BsCand gm[GROUPS];
   __shared__ BsCand buf[BS_CAP];
   __shared__ BsCand bound;
   __shared__ BsCand wbest[BS_THREADS / 32];
   __shared__ int count;
-  pdl_wait();
-  pdl_launch_dependents();
   const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t row0 = (size_t)s * B;
+  const int total = B * parts * n;
   const BsCand none = {-INFINITY, 0xffffffffu};
-  // a warp per row: its maximum, its sum, the entries with weight exchanged for their exp in 64 bits
+  if (tid == 0) count = 0;
+  pdl_wait();
+  pdl_launch_dependents();
+  // candidate i: its value without its beam's share, and which beam's; everything is on its way before the first is waited for
+  struct Raw {
+    float x, score;
+    int beam;                             // -1: none
+    uint32_t token;
+  };
+  auto raw = [&](int i) -> Raw {
+    if (i >= total) return {0.0f, 0.0f, -1, 0u};
+    const int k = i / n, b = k / parts;
+    const uint2 c = cand[row0 * parts * n + i];
+    return {bs_value(c.x), scores[row0 + b], i - k * n < part[row0 * parts + k].count ? b : -1, c.y};
+  };
+  auto value = [&](const Raw& r) -> BsCand {
+    if (r.beam < 0) return none;
+    return {(double)r.score + ((double)r.x - lse[r.beam]), (uint32_t)r.beam * (uint32_t)V + r.token};
+  };
+  Raw held[HELD];
+  if (CAND) {
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) held[j] = raw(tid + j * BS_THREADS);
+  }
+  // a warp per row: its maximum, its sum
   for (int b = warp; b < B; b += BS_THREADS / 32) {
     const BsPart* p = part + (row0 + b) * parts;
-    float M = -INFINITY;
-    for (int i = lane; i < parts; i += 32) M = fmaxf(M, p[i].max);
+    BsPart q = {0.0, -INFINITY, 0};
+    if (lane < parts) q = p[lane];
+    float M = q.max;
+    for (int i = lane + 32; i < parts; i += 32) M = fmaxf(M, p[i].max);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if (M == -INFINITY) {
-      if (lane == 0) base[b] = -INFINITY;
-      continue;
-    }
     double sum = 0.0;
-    for (int i = lane; i < parts; i += 32)
-      if (p[i].count) sum += p[i].sum * exp((double)p[i].max - (double)M);
-    const uint2* c = cand + (row0 + b) * parts * n;
-    for (int i = lane; i < parts * n; i += 32) {
-      const int k = i / n;
-      const BsPart q = p[k];
-      if (i - k * n < q.count) {
-        const float x = bs_value(c[i].x);
-        // (a part far below the row's maximum has no weight; neither has an entry 2^-20 of it)
-        if (x - M > -14.0f) sum += exp((double)x - (double)M) - (double)bs_exp(x, q.max) * exp((double)q.max - (double)M);
-      }
+    for (int i = lane; i < parts; i += 32) {
+      if (i >= 32) q = p[i];
+      if (q.count) sum += q.max == M ? q.sum : q.sum * exp((double)q.max - (double)M);
     }
+    if (parts > 1) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) base[b] = (double)M + log(sum);      // lse
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    if (lane == 0) lse[b] = (double)M + log(sum);       // (a row without entries: not used)
   }
-  if (tid == 0) count = 0;
   __syncthreads();
-  const int total = B * parts * n;
-  auto entry = [&](int i) -> BsCand {
-    const int k = i / n, b = k / parts;
-    if (i - k * n >= part[row0 * parts + k].count) return none;
-    const uint2 c = cand[row0 * parts * n + i];
-    return {(double)scores[row0 + b] + ((double)bs_value(c.x) - base[b]), (uint32_t)b * (uint32_t)V + c.y};
-  };
-  BsCand best = none;
-  for (int i = tid; i < total; i += BS_THREADS) {
-    const BsCand e = entry(i);
-    if (bs_before(e, best)) best = e;
+  BsCand mine[HELD], best = none;
+  if (CAND) {
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+      mine[j] = value(held[j]);
+      if (bs_before(mine[j], best)) best = mine[j];
+    }
+  } else {
+    for (int i = tid; i < total; i += BS_THREADS) {
+      const BsCand e = value(raw(i));
+      if (bs_before(e, best)) best = e;
+    }
   }
 #pragma unroll
   for (int o = 1; o < GS; o <<= 1) {
@@ -265,44 +421,54 @@ beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ can
   if (tid % GS == 0) gm[tid / GS] = best;
   __syncthreads();
   if (tid < GROUPS) {
-    const BsCand mine = gm[tid];
+    const BsCand of = gm[tid];
     int rank = 0;
 #pragma unroll 4
-    for (int k = 0; k < GROUPS; ++k) rank += bs_before(gm[k], mine) || (k < tid && gm[k].at == mine.at) ? 1 : 0;   // (empty groups are equal)
-    if (rank == (n < GROUPS ? n : GROUPS) - 1) bound = mine;
+    for (int k = 0; k < GROUPS; ++k) rank += bs_before(gm[k], of) || (k < tid && gm[k].at == of.at) ? 1 : 0;   // (empty groups are equal)
+    if (rank == (n < GROUPS ? n : GROUPS) - 1) bound = of;
   }
   __syncthreads();
   const BsCand bd = bound;
-  for (int i = tid; i < total; i += BS_THREADS) {
-    const BsCand e = entry(i);
+  auto collect = [&](const BsCand& e) {
     if (e.at != 0xffffffffu && !bs_before(bd, e)) {
       const int at = atomicAdd(&count, 1);
       if (at < BS_CAP) buf[at] = e;
     }
+  };
+  if (CAND) {
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) collect(mine[j]);
+  } else {
+    for (int i = tid; i < total; i += BS_THREADS) collect(value(raw(i)));
   }
   __syncthreads();
   const int c = count;
   const size_t o0 = (size_t)s * n;
   auto put = [&](int r, const BsCand& e) {
     const bool got = e.at != 0xffffffffu && e.v > -INFINITY;
+    const uint32_t beam = e.at / (uint32_t)V;
     values[o0 + r] = got ? (float)e.v : -INFINITY;
-    beams[o0 + r] = got ? (int)(e.at / (uint32_t)V) : -1;
-    tokens[o0 + r] = got ? (int)(e.at % (uint32_t)V) : -1;
+    beams[o0 + r] = got ? (int)beam : -1;
+    tokens[o0 + r] = got ? (int)(e.at - beam * (uint32_t)V) : -1;
   };
-  if (c <= BS_CAP) {
-    for (int i = tid; i < c; i += BS_THREADS) {
-      const BsCand mine = buf[i];
-      int rank = 0;
-      for (int k = 0; k < c; ++k) rank += bs_before(buf[k], mine) ? 1 : 0;
-      if (rank < n) put(rank, mine);
+  if (CAND || c <= BS_CAP) {              // (held candidates are at most as many as there is room for)
+    for (int i = tid; i < max(c, n); i += BS_THREADS) {
+      BsCand e = none;
+      int rank = i;                       // places without a candidate
+      if (i < c) {
+        e = buf[i];
+        rank = 0;
+        for (int k = 0; k < c; ++k) rank += bs_before(buf[k], e) ? 1 : 0;
+      }
+      if (rank < n) put(rank, e);
     }
-    for (int r = c + tid; r < n; r += BS_THREADS) put(r, none);
   } else {
+    // more reach the bound than there is room for (they bunch in few threads): one after the other
     BsCand last = {INFINITY, 0u};
     for (int r = 0; r < n; ++r) {
       BsCand m = none;
       for (int i = tid; i < total; i += BS_THREADS) {
-        const BsCand e = entry(i);
+        const BsCand e = value(raw(i));
         if (e.at != 0xffffffffu && (r == 0 || bs_before(last, e)) && bs_before(e, m)) m = e;
       }
 #pragma unroll
@@ -322,32 +488,34 @@ beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ can
   }
 }
 
-// Entries per thread: the fewest (the most blocks) that leave at most eight blocks of a row or so on each of 148 SMs.
-static int bs_entries(int rows, int V) {
-  for (int e = 4; e < 32; e *= 2)
-    if ((long long)rows * ((V + BS_THREADS * e - 1) / (BS_THREADS * e)) <= 148 * 8) return e;
-  return 32;
+// Entries of a row per block: the fewest tiles (the most blocks) that leave at most as many blocks as run at once on 148 SMs; BS_MAX_TILES at
+// most.
+static int bs_chunk(int rows, int V) {
+  for (int tiles = 1; tiles < BS_MAX_TILES; tiles *= 2)
+    if ((long long)rows * ((V + BS_TILE * tiles - 1) / (BS_TILE * tiles)) <= 148 * BS_PER_SM) return BS_TILE * tiles;
+  return BS_TILE * BS_MAX_TILES;
 }
-static int bs_parts(int V, int e) { return (int)(((long long)V + 3 + BS_THREADS * e - 1) / (BS_THREADS * e)); }   // + 3: a shifted row
+// (rows that do not begin on 16-byte boundaries are shifted by up to three entries)
+static int bs_parts(int V, int chunk, bool shifted) { return (int)(((long long)V + (shifted ? 3 : 0) + chunk - 1) / chunk); }
 
 extern "C" long long tl_beam_scratch_bytes(int rows, int V, int n) {
-  return (long long)rows * bs_parts(V, bs_entries(rows, V)) * ((long long)sizeof(BsPart) + 8 * n);
+  return (long long)rows * bs_parts(V, bs_chunk(rows, V), true) * ((long long)sizeof(BsPart) + 8 * n);
 }
 
 template <int GS>
 static int bs_run(const float* logits, long long ld, int S, int B, int V, const float* scores, int n, void* scratch, float* values,
                   int* beams, int* tokens, cudaStream_t stream) {
-  const int rows = S * B, e = bs_entries(rows, V), parts = bs_parts(V, e);
+  const int rows = S * B, chunk = bs_chunk(rows, V), parts = bs_parts(V, chunk, ld % 4 != 0 || ((uintptr_t)logits & 15));
   BsPart* part = (BsPart*)scratch;
   uint2* cand = (uint2*)(part + (size_t)rows * parts);
-  const dim3 grid(parts, rows), block(BS_THREADS);
-  const int st = e == 4    ? tl_launch(beam_rows_kernel<4, GS>, grid, block, 0, stream, logits, ld, V, scores, n, parts, part, cand)
-                 : e == 8  ? tl_launch(beam_rows_kernel<8, GS>, grid, block, 0, stream, logits, ld, V, scores, n, parts, part, cand)
-                 : e == 16 ? tl_launch(beam_rows_kernel<16, GS>, grid, block, 0, stream, logits, ld, V, scores, n, parts, part, cand)
-                           : tl_launch(beam_rows_kernel<32, GS>, grid, block, 0, stream, logits, ld, V, scores, n, parts, part, cand);
+  const int st = tl_launch(beam_rows_kernel<GS>, dim3(parts, rows), dim3(BS_THREADS), 0, stream, logits, ld, V, scores, n, chunk, part, cand);
   if (st) return st;
-  return tl_launch(beam_merge_kernel<GS>, dim3(S), block, (size_t)B * sizeof(double), stream, (const BsPart*)part, (const uint2*)cand,
-                   scores, B, V, n, parts, values, beams, tokens);
+  const long long total = (long long)B * parts * n;
+  auto merge = [&](auto kernel) {
+    return tl_launch(kernel, dim3(S), dim3(BS_THREADS), (size_t)B * sizeof(double), stream, (const BsPart*)part, (const uint2*)cand, scores, B,
+                     V, n, parts, values, beams, tokens);
+  };
+  return total <= BS_THREADS ? merge(beam_merge_kernel<GS, 1>) : total <= 4 * BS_THREADS ? merge(beam_merge_kernel<GS, 4>) : merge(beam_merge_kernel<GS, 0>);
 }
 
 // logits [S * B] rows of V entries, `ld` apart; scores [S * B]; values, beams, tokens [S * n].  `scratch`: tl_beam_scratch_bytes,
@@ -358,7 +526,7 @@ extern "C" int tl_beam_select(const float* logits, long long ld, int S, int B, i
   if (B <= 0 || V <= 0 || n <= 0 || ld < V || ((uintptr_t)logits & 3)) return -1;
   if (V > (1 << 30)) return -2;
   if (n > BS_MAX_N || B > 1024 || (long long)S * B > 65535 || (long long)B * V >= 0x7fffffffLL ||
-      (long long)B * bs_parts(V, 4) * n >= 0x7fffffffLL)
+      (long long)B * bs_parts(V, BS_TILE, true) * n >= 0x7fffffffLL)
     return -2;
   // twice as many groups as entries are asked for, where there are
   if (n <= 16) return bs_run<8>(logits, ld, S, B, V, scores, n, scratch, values, beams, tokens, stream);

@@ -6,6 +6,7 @@ a CUDA device, a missing library or a launch that the driver rejects raises
 """
 from __future__ import annotations
 
+from array import array
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Callable, Dict, Optional, Sequence
 
@@ -124,12 +125,19 @@ def _need(t: torch.Tensor, dtype: torch.dtype, what: str, contiguous: bool = Tru
         raise KernelError(f"{what}: tensor must be contiguous")
 
 
-def _here(t: torch.Tensor, what: str) -> None:
-    """Kernels are launched on the current device's current stream: their tensors must lie there."""
-    if not t.is_cuda:
+def _here(t: torch.Tensor, what: str) -> int:
+    """Kernels are launched on the current device's current stream: their tensors must lie there.  Returns the device."""
+    i = t.get_device()
+    if i < 0:
         raise KernelError(f"{what}: tensor is not on a CUDA device; this package has no CPU path")
-    if t.device.index != torch.cuda.current_device():
+    if i != torch._C._cuda_getDevice():
         raise KernelError(f"{what}: tensor lies on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return i
+
+
+def _stream_on(device: int) -> int:
+    """The handle of the current stream of a device that `_here` has returned."""
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def _pairs(src: Sequence[int], dst: Sequence[int], limit: int, what: str) -> int:
@@ -172,6 +180,9 @@ class CoreOps:
             fn = getattr(self.lib, f"{base}_{self.suffix}")
             fn.restype = c_int
             setattr(self, "_" + base, fn)
+        P, I, L = c_void_p, c_int, c_longlong
+        self._tl_copy_slots.argtypes = [P, I, I, L, P, P, I, P]
+        self._tl_copy_pages.argtypes = [P, I, L, I, I, I, I, P, P, P, I, P]
 
     # x[t, :] = table[tokens[t], :]
     def embed(self, tokens: torch.Tensor, table: torch.Tensor, x: torch.Tensor,
@@ -1312,23 +1323,25 @@ class CoreOps:
     def copy_slots(self, storage: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> None:
         """Row dst[i] of every layer of `storage` ([layers, slots, ...], any type) becomes what row src[i] holds.
         No row may be written twice or be written and read."""
-        _here(storage, "copy_slots")
+        dev = _here(storage, "copy_slots")
         if storage.dim() < 2 or not storage.is_contiguous():
             raise KernelError("copy_slots: the storage must be contiguous [layers, slots, ...]")
         n = _pairs(src, dst, storage.shape[1], "copy_slots: slot")
-        if n == 0 or storage.numel() == 0:
+        numel = storage.numel()
+        if n == 0 or numel == 0:
             return
         layers, slots = storage.shape[0], storage.shape[1]
-        row = storage.numel() // (layers * slots) * storage.element_size()
-        _check(self._tl_copy_slots(_ptr(storage), c_int(layers), c_int(slots), c_longlong(row), (c_int * n)(*src),
-                                   (c_int * n)(*dst), c_int(n), _stream()), "copy_slots")
+        lists = array("i", [*src, *dst])
+        at = lists.buffer_info()[0]
+        _check(self._tl_copy_slots(storage.data_ptr(), layers, slots, numel // (layers * slots) * storage.element_size(), at,
+                                   at + 4 * n, n, _stream_on(dev)), "copy_slots")
 
     def copy_pages(self, storage: torch.Tensor, pages: int, heads: int, dim: int, vdim: int, src: Sequence[int],
                    dst: Sequence[int], counts: Sequence[int]) -> None:
         """The first counts[i] positions of page src[i] into page dst[i], in every layer of `storage` ([layers, n]: per
         layer the key pages [pages, heads, PAGE, dim], then the value pages [pages, heads, vdim, PAGE]; vdim 0: none).
         Later positions of dst[i] keep what they hold.  No page may be written twice or be written and read."""
-        _here(storage, "copy_pages")
+        dev = _here(storage, "copy_pages")
         _need(storage, self.act_dtype, "copy_pages storage")
         if storage.dim() != 2 or min(pages, heads, dim) < 1 or vdim < 0 or \
                 storage.shape[1] < pages * heads * PAGE * (dim + vdim):
@@ -1338,9 +1351,10 @@ class CoreOps:
             raise KernelError(f"copy_pages: one count of 1 to {PAGE} positions per pair is needed")
         if n == 0 or storage.shape[0] == 0:
             return
-        _check(self._tl_copy_pages(_ptr(storage), c_int(storage.shape[0]), c_longlong(storage.shape[1]), c_int(pages),
-                                   c_int(heads), c_int(dim), c_int(vdim), (c_int * n)(*src), (c_int * n)(*dst),
-                                   (c_int * n)(*counts), c_int(n), _stream()), "copy_pages")
+        lists = array("i", [*src, *dst, *counts])
+        at = lists.buffer_info()[0]
+        _check(self._tl_copy_pages(storage.data_ptr(), storage.shape[0], storage.shape[1], pages, heads, dim, vdim, at, at + 4 * n,
+                                   at + 8 * n, n, _stream_on(dev)), "copy_pages")
 
 
 class BeamOps:
@@ -1352,36 +1366,46 @@ class BeamOps:
         P, I, L = c_void_p, c_int, c_longlong
         self._scratch = lib.tl_beam_scratch_bytes
         self._scratch.restype, self._scratch.argtypes = L, [I, I, I]
+        self._sizes: Dict[tuple, int] = {}       # scratch bytes by (rows, vocabulary, n)
         self._select = lib.tl_beam_select
         self._select.restype, self._select.argtypes = I, [P, L, I, I, I, P, I, P, P, P, P, P]
 
     def select(self, logits: torch.Tensor, scores: torch.Tensor, n: int) -> torch.Tensor:
-        """logits [S * B, V], scores [S, B], both 32-bit.  Returns int32 [3, S, n]: the bits of the values (32-bit
-        floats), the beams, the tokens."""
-        _here(logits, "beam select")
-        _here(scores, "beam select")
+        """logits [S * B, V], scores [S, B], both 32-bit.  Returns int32 [3 or more, S, n]: the bits of the values (32-bit
+        floats), the beams, the tokens; what follows is scratch."""
+        dev = _here(logits, "beam select")
+        if scores.get_device() != dev:
+            raise KernelError(f"beam select: the scores lie on {scores.device}, the logits on {logits.device}")
         if logits.dtype != torch.float32 or scores.dtype != torch.float32:
             raise KernelError("beam select: logits and scores must be 32-bit floats")
         if logits.dim() != 2 or scores.dim() != 2 or logits.shape[0] != scores.numel():
             raise KernelError("beam select: logits [sequences * beams, vocabulary] and scores [sequences, beams] are needed, "
                               f"got {tuple(logits.shape)} and {tuple(scores.shape)}")
-        V = logits.shape[1]
-        if (V > 1 and logits.stride(1) != 1) or not scores.is_contiguous():
-            raise KernelError("beam select: scores and the rows of logits must be contiguous")
+        rows, V = logits.shape
         S, B = scores.shape
+        ld, step = logits.stride()
+        if (V > 1 and step != 1) or not scores.is_contiguous():
+            raise KernelError("beam select: scores and the rows of logits must be contiguous")
         if S and not 1 <= n <= min(self.MAX_N, B * V):
             raise KernelError(f"beam select: {n} continuations of {B} beams and {V} tokens (1 to {self.MAX_N} are possible)")
-        ld = logits.stride(0) if S * B > 1 else V
+        if rows <= 1:
+            ld = V
         if ld < V:
             raise KernelError("beam select: the rows of logits overlap")
-        out = torch.empty((3, S, n), dtype=torch.int32, device=logits.device)
         if S == 0:
-            return out
-        # a buffer of this call's own: calls on other streams and recorded graphs share nothing
-        scratch = torch.empty(self._scratch(S * B, V, n), dtype=torch.uint8, device=logits.device)
+            return torch.empty((3, 0, n), dtype=torch.int32, device=logits.device)
+        # One buffer of this call's own for the result and, behind it, what the kernels need: calls on other streams and recorded
+        # graphs share nothing.
+        size = self._sizes.get((rows, V, n))
+        if size is None:
+            if len(self._sizes) > 4096:
+                self._sizes.clear()
+            size = self._sizes[rows, V, n] = self._scratch(rows, V, n)
+        more = -(-(size + 16) // (4 * S * n))
+        out = logits.new_empty((3 + more, S, n), dtype=torch.int32)
         at = out.data_ptr()
-        _check(self._select(logits.data_ptr(), ld, S, B, V, scores.data_ptr(), n, scratch.data_ptr(), at, at + 4 * S * n,
-                            at + 8 * S * n, _stream()), "beam_select")
+        _check(self._select(logits.data_ptr(), ld, S, B, V, scores.data_ptr(), n, (at + 12 * S * n + 15) & ~15, at, at + 4 * S * n,
+                            at + 8 * S * n, _stream_on(dev)), "beam_select")
         return out
 
 
