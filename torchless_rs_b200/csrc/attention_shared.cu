@@ -170,8 +170,8 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   uint64_t* q_full = pv_done + 2;                      // [2]
   uint64_t* o_free = q_full + 2;
   uint32_t* tmem_slot = (uint32_t*)(o_free + 1);
-  int* total_s = (int*)(tmem_slot + 1);                // [2]: tiles in the line, tiles of the longest unit
-  volatile int* abort_flag = (volatile int*)(total_s + 2);
+  int* total_s = (int*)(tmem_slot + 1);                // [3]
+  volatile int* abort_flag = (volatile int*)(total_s + 3);
   // [2][3]: a reference in this half of the columns has to move.  By tile number modulo 3: written before a tile's barrier, read after
   // it, cleared behind the next one (what a warp that runs ahead writes by then is another tile's).
   volatile int* moved_s = abort_flag + 1;
@@ -201,12 +201,12 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   }
   pdl_wait();
   pdl_launch_dependents();
-  if (warp == 8) sh_make_line<2>(table, total_s, a, lane);
+  if (warp == 8) sh_make_line<2>(table, total_s, a, gridDim.x, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot, tmem_o = tmem + 2 * N;
-  const int total = total_s[0], share = sh_share(total_s, gridDim.x, a.parts);
+  const int total = total_s[0], gap = total_s[2], share = sh_share(total_s, gridDim.x, a.parts);
   const int t0 = min((int)blockIdx.x * share, total), t1 = min(t0 + share, total);
   const int G = a.nh / a.nkv;
 
@@ -216,9 +216,9 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       bool ok = true;
       int n = 0;
       for (int t = t0; t < t1 && ok;) {
-        const ShPiece p = sh_locate<2>(table, a, t);
-        const int last = min(p.tiles, p.tile + t1 - t);
-        for (int j = p.tile; j < last && ok; ++j, ++t, ++n) {
+        const ShPiece p = sh_locate(table, a, gap, t, t1);
+        t = p.next;
+        for (int j = p.tile; j < p.last && ok; ++j, ++n) {
           const int pages = min(2, p.pages - 2 * j);
           int slab[2];
           for (int h = 0; h < pages; ++h) {
@@ -256,23 +256,31 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       auto lo_of = [](const uint8_t* s) { return ((smem_u32(s) & 0x3FFFFu) >> 4) | (1u << 16); };
       auto desc = [&](uint32_t lo) { return ((uint64_t)desc_hi << 32) | lo; };
       const uint32_t k_lo = lo_of(k_s), v_lo = lo_of(v_s), q_lo = lo_of(q_s), p_lo = lo_of(p_s);
-      const int tiles = t1 - t0;
-      bool ok = true;
       // tile n + 1's unit runs ahead of tile n's
-      int s_unit = 0, s_left = 0, s_t = t0;       // for S^T: units begun, tiles left of the current one
+      int s_unit = 0, s_left = 0, s_t = t0;       // for S^T: units begun, tiles left of the current one, the next piece's place
       int o_unit = 0, o_left = 0, o_t = t0, o_tile = 0;
       ShPiece o_piece = {};
       bool o_first = false;
+      auto piece = [&](int& t) {                  // the next piece with tiles; without, if there is none
+        ShPiece p = {};
+        while (t < t1) {
+          p = sh_locate(table, a, gap, t, t1);
+          t = p.next;
+          if (p.tile < p.last) break;
+        }
+        return p;
+      };
+      // 1: issued, 0: there is no further tile, -1: given up
       auto scores = [&](int n) {
         if (s_left == 0) {
-          const ShPiece p = sh_locate<2>(table, a, s_t);
-          s_left = min(p.tiles - p.tile, t1 - s_t);
-          s_t += s_left;
-          if (!sh_park(&q_full[s_unit & 1], (uint32_t)(s_unit >> 1) & 1u, abort_flag, 3)) return false;
+          const ShPiece p = piece(s_t);
+          s_left = p.last - p.tile;
+          if (s_left == 0) return 0;
+          if (!sh_park(&q_full[s_unit & 1], (uint32_t)(s_unit >> 1) & 1u, abort_flag, 3)) return -1;
           ++s_unit;
         }
         --s_left;
-        if (!sh_park(&k_full[n % Z::KS], (uint32_t)(n / Z::KS) & 1u, abort_flag, 4)) return false;
+        if (!sh_park(&k_full[n % Z::KS], (uint32_t)(n / Z::KS) & 1u, abort_flag, 4)) return -1;
         tc_fence_after();
         const uint32_t ka = k_lo + (uint32_t)(n % Z::KS) * (Z::K >> 4), qa = q_lo + (uint32_t)((s_unit - 1) & 1) * (Z::Q >> 4);
 #pragma unroll
@@ -281,15 +289,15 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
                     desc(qa + (kk >> 2) * ((N * 128) >> 4) + (kk & 3) * 2), idesc, kk > 0 ? 1u : 0u);
         umma_commit(&s_full[n & 1]);
         umma_commit(&k_empty[n % Z::KS]);
-        return true;
+        return 1;
       };
-      ok = scores(0);
-      for (int n = 0; n < tiles && ok; ++n) {
-        if (n + 1 < tiles && !scores(n + 1)) break;     // (its buffer was read before P of tile n - 1 was there)
+      int ready = scores(0);                      // whether tile n's scores have been issued
+      for (int n = 0; ready == 1; ++n) {
+        ready = scores(n + 1);                    // (its buffer was read before P of tile n - 1 was there)
+        if (ready < 0) break;
         if (o_left == 0) {
-          o_piece = sh_locate<2>(table, a, o_t);
-          o_left = min(o_piece.tiles - o_piece.tile, t1 - o_t);
-          o_t += o_left;
+          o_piece = piece(o_t);
+          o_left = o_piece.last - o_piece.tile;
           o_tile = o_piece.tile;
           o_first = true;
           // O^T is free when the unit before has been written out
@@ -322,13 +330,18 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       volatile int* moved = moved_s + 3 * upper;
       const int my_col = first_col + (key & (NC - 1)), my_beam = my_col / G, my_head = my_col - my_beam * G;
       const int first_beam = first_col / G, first_head = first_col - first_beam * G;
+      const ShRow q_row(tid / (HEAD_DIM / 8), G);
       auto load_q = [&](const ShPiece& p, int buf) {
         uint8_t* dst = q_s + buf * Z::Q;
-        for (int i = tid; i < N * (HEAD_DIM / 8); i += SH_SOFT) {
-          const int r = i / (HEAD_DIM / 8), c = i % (HEAD_DIM / 8);
+        constexpr int C = HEAD_DIM / 8;        // 16-byte pieces of a row
+        const int c = tid % C;
+        ShRow at = q_row;
+#pragma unroll 1
+        for (int r = tid / C; r < N; r += SH_SOFT / C) {
           uint4 v = make_uint4(0, 0, 0, 0);
-          if (r < p.beams * G) v = ldg16(a.q + ((size_t)(p.row0 + r / G) * a.nh + p.kvh * G + r % G) * HEAD_DIM + c * 8);
+          if (r < p.beams * G) v = ldg16(a.q + ((size_t)(p.row0 + at.beam) * a.nh + p.kvh * G + at.head) * HEAD_DIM + c * 8);
           *reinterpret_cast<uint4*>(dst + (c >> 3) * (N * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+          at.step(SH_SOFT / C);
         }
         sh_async_fence();
         sh_arrive(&q_full[buf]);
@@ -342,12 +355,21 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           neg_ref[c] = r.x; neg_ref[c + 1] = r.y; neg_ref[c + 2] = r.z; neg_ref[c + 3] = r.w;
         }
       };
-      ShPiece p = sh_locate<2>(table, a, t0);
-      load_q(p, 0);
-      for (int t = t0; t < t1; ++unit) {
-        const int last = min(p.tiles, p.tile + t1 - t), R = p.beams * G;
-        const int next = t + last - p.tile;
-        ShPiece np = p;
+      int t = t0;
+      auto piece = [&] {                       // the next piece with tiles; without, if there is none
+        ShPiece p = {};
+        while (t < t1) {
+          p = sh_locate(table, a, gap, t, t1);
+          t = p.next;
+          if (p.tile < p.last) break;
+        }
+        return p;
+      };
+      ShPiece p = piece();
+      if (p.tile < p.last) load_q(p, 0);
+      for (; p.tile < p.last; ++unit) {
+        const int last = p.last, R = p.beams * G;
+        ShPiece np = {};
 #pragma unroll
         for (int c = 0; c < NC; ++c) l[c] = neg_ref[c] = 0.0f;
         if (key < NC) {
@@ -457,10 +479,10 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           sh_async_fence();
           tc_fence_before();
           sh_arrive(&p_full[buf]);
-          if (j == p.tile && next < t1) {
+          if (j == p.tile) {
             // the next unit's queries: its buffer's scores were all read a unit ago
-            np = sh_locate<2>(table, a, next);
-            load_q(np, (unit + 1) & 1);
+            np = piece();
+            if (np.tile < np.last) load_q(np, (unit + 1) & 1);
           }
           // two pages on
 #pragma unroll
@@ -509,7 +531,6 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         tc_fence_before();
         sh_arrive(o_free);
         sh_bar(upper);                         // red_s and ref_s are written again
-        t = next;
         p = np;
       }
     }

@@ -21,6 +21,9 @@ static_assert(PAGE == 64, "the tiles are laid out for pages of 64 tokens");
 
 #define SH_MAX_PARTS 160
 #define SH_MAX_GROUPS 256
+#ifndef SH_UNIT_TILES
+#define SH_UNIT_TILES 4
+#endif
 
 template <typename T>
 struct ShArgs {
@@ -55,79 +58,110 @@ __device__ __forceinline__ ShSpan sh_span(int len, int window, int shared) {
 }
 struct ShGroup {
   int before;                  // tiles of the groups before
-  int row0, rows, len, lo, first, common, own;
+  int row0, len, lo, first, common, own;
+  int full, rest;              // units with all their rows (per kv head), rows of a last one with fewer
+  int t_full, t_rest, per_kv;  // tiles of either; places that a kv head takes in the line
 };
-// A stretch of a unit's tiles.
+// What a stretch has of a unit.
 struct ShPiece {
   int kvh, row0, beams, len, lo, first, common, own, pages;
-  int tile, tiles;             // the first tile of the stretch, tiles of the unit
-  int unit, start;             // the unit's number, its first tile in the line
+  int tile, last, tiles;       // tiles [tile, last) of the unit's `tiles`; none if tile == last
+  int unit, start, next;       // the unit's number; the places in the line of its first tile and of what follows this piece
 };
 
 // TP: pages of a tile
 template <int TP>
 __device__ __forceinline__ int sh_tiles(int common, int own, int beams) { return (common + own * beams + TP - 1) / TP; }
 
-// One warp: the groups' places in the line.  totals: tiles in the line, tiles of the longest unit.
+// One warp: the groups' places in the line.  Every unit begins with `totals[2]` places without a tile: that is what beginning a unit and
+// writing one out takes a block, in tiles, so that equal stretches take equal time (22B sizes, 4 prompts x 8 beams: blocks with one unit
+// 39 us and with two 50 us without them).  Where a stretch is a few tiles long there are none: more, shorter stretches are then
+// faster.  totals[0], [1]: places in the line, tiles of the longest unit.
 template <int TP, typename T>
-__device__ __forceinline__ void sh_make_line(ShGroup* table, int* totals, const ShArgs<T>& a, int lane) {
-  int before = 0, longest = 0;
+__device__ __forceinline__ void sh_make_line(ShGroup* table, int* totals, const ShArgs<T>& a, int blocks, int lane) {
+  int tiles = 0, units = 0, longest = 0;
   for (int g0 = 0; g0 < a.groups; g0 += 32) {
     const int g = g0 + lane;
     ShGroup e = {};
-    int n = 0;
+    int n = 0, u = 0;
     if (g < a.groups) {
       e.row0 = a.group_start[g];
-      e.rows = a.group_start[g + 1] - e.row0;
-      if (e.rows > 0) {
+      const int rows = a.group_start[g + 1] - e.row0;
+      if (rows > 0) {
         const ShSpan s = sh_span(a.seq_len[e.row0], a.window, a.group_pages[g]);
         e.len = s.len; e.lo = s.lo; e.first = s.first; e.common = s.common; e.own = s.own;
-        const int full = e.rows / a.beams, rest = e.rows - full * a.beams;
-        n = a.nkv * (full * sh_tiles<TP>(s.common, s.own, a.beams) + (rest ? sh_tiles<TP>(s.common, s.own, rest) : 0));
-        longest = max(longest, sh_tiles<TP>(s.common, s.own, min(e.rows, a.beams)));
+        if (s.common + s.own > 0) {
+          e.full = a.row_blocks == 1 && rows == a.beams ? 1 : rows / a.beams;
+          e.rest = rows - e.full * a.beams;
+          e.t_full = sh_tiles<TP>(s.common, s.own, a.beams);
+          e.t_rest = e.rest ? sh_tiles<TP>(s.common, s.own, e.rest) : 0;
+          n = a.nkv * (e.full * e.t_full + e.t_rest);
+          u = a.nkv * (e.full + (e.rest ? 1 : 0));
+          longest = max(longest, e.full ? e.t_full : e.t_rest);
+        }
       }
     }
-    int sum = n;
+    int sum = n, sum_u = u;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += v;
+      const int v = __shfl_up_sync(0xffffffffu, sum, o), w = __shfl_up_sync(0xffffffffu, sum_u, o);
+      if (lane >= o) { sum += v; sum_u += w; }
     }
-    e.before = before + sum - n;
+    e.before = tiles + sum - n;
+    e.per_kv = units + sum_u - u;         // (units before, for now)
     if (g < a.groups) table[g] = e;
-    before += __shfl_sync(0xffffffffu, sum, 31);
+    tiles += __shfl_sync(0xffffffffu, sum, 31);
+    units += __shfl_sync(0xffffffffu, sum_u, 31);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-  if (lane == 0) { totals[0] = before; totals[1] = longest; }
+  const int gap = min(SH_UNIT_TILES, (tiles + blocks - 1) / blocks / 3);
+  for (int g = lane; g < a.groups; g += 32) {
+    ShGroup& e = table[g];
+    e.before += gap * e.per_kv;
+    e.per_kv = e.full * (e.t_full + gap) + (e.rest ? e.t_rest + gap : 0);
+  }
+  if (lane == 0) { totals[0] = tiles + gap * units; totals[1] = longest; totals[2] = gap; }
 }
 // The length of a stretch: an equal share, but no unit in more pieces than there is room for.
 __device__ __forceinline__ int sh_share(const int* totals, int blocks, int parts) {
   return max((totals[0] + blocks - 1) / blocks, (totals[1] + parts - 2) / (parts - 1));
 }
 
-template <int TP, typename T>
-__device__ ShPiece sh_locate(const ShGroup* table, const ShArgs<T>& a, int t) {
+// The rows of a unit one after the other, as a row of the group and a query head of the kv head's.
+struct ShRow {
+  int beam, head, G;
+  __device__ __forceinline__ ShRow(int r, int G_) : G(G_) { beam = r / G; head = r - beam * G; }
+  __device__ __forceinline__ void step(int k) {
+    head += k;
+    while (head >= G) { head -= G; ++beam; }
+  }
+};
+
+// What the stretch that ends at t1 has at place t.
+template <typename T>
+__device__ ShPiece sh_locate(const ShGroup* table, const ShArgs<T>& a, int gap, int t, int t1) {
   int lo = 0, hi = a.groups - 1;
   while (lo < hi) {            // the last group that begins at or before t and has tiles
     const int mid = (lo + hi + 1) >> 1;
     if (table[mid].before <= t) lo = mid; else hi = mid - 1;
   }
   const ShGroup& g = table[lo];
-  const int full = g.rows / a.beams, rest = g.rows - full * a.beams;
-  const int t_full = sh_tiles<TP>(g.common, g.own, a.beams), t_rest = rest ? sh_tiles<TP>(g.common, g.own, rest) : 0;
-  const int per_kv = full * t_full + t_rest, in_group = t - g.before, kvh = in_group / per_kv, r = in_group - kvh * per_kv;
-  const int rb = min(r / t_full, full), j = r - rb * t_full;
+  const int in_group = t - g.before, kvh = in_group / g.per_kv, r = in_group - kvh * g.per_kv;
+  const int rb = a.row_blocks == 1 ? 0 : min(r / (g.t_full + gap), g.full), j = r - rb * (g.t_full + gap);
+  const bool whole = rb < g.full;
   ShPiece p;
   p.kvh = kvh;
   p.row0 = g.row0 + rb * a.beams;
-  p.beams = rb < full ? a.beams : rest;
+  p.beams = whole ? a.beams : g.rest;
   p.len = g.len; p.lo = g.lo; p.first = g.first; p.common = g.common; p.own = g.own;
   p.pages = g.common + g.own * p.beams;
-  p.tile = j;
-  p.tiles = rb < full ? t_full : t_rest;
+  p.tiles = whole ? g.t_full : g.t_rest;
   p.unit = (lo * a.row_blocks + rb) * a.nkv + kvh;
-  p.start = t - j;
+  p.start = t - j + gap;
+  p.tile = max(j - gap, 0);
+  p.next = min(p.start + p.tiles, t1);
+  p.last = max(p.next - p.start, p.tile);
   return p;
 }
 // Page i of a unit: the row (of the unit) whose table and weights it takes, -1 for a common one, and the table's column.

@@ -17,6 +17,7 @@ MAX_GROUPS = 256               # groups of one call
 MAX_HEADS = {torch.bfloat16: 16, torch.float32: 32}     # query heads per key/value head
 BLOCK_ROWS = {torch.bfloat16: 64, torch.float32: 32}    # rows of a unit (rows of a group, times query heads)
 TILE_PAGES = {torch.bfloat16: 2, torch.float32: 1}      # pages that a block takes at a time
+PER_SM = {torch.bfloat16: 1, torch.float32: 2}          # resident blocks
 MAX_PARTS = 160                # pieces of a unit that the merge takes
 
 for _hd in HEAD_DIMS:
@@ -133,7 +134,7 @@ class SharedAttention:
             raise KernelError(f"shared attention: a window of {window}")
         if self._call is None:
             self._load()
-        blocks = _sm_count(dev)
+        blocks = _sm_count(dev) * PER_SM[self.dtype]
         row_blocks, parts = shared_plan(tuple(lens), tuple(shared), group_rows, nkv, nh // nkv, window or 0, self.dtype, blocks, bound)
         part = workspace.get("attn_shared_part", (rows * nh * parts * (hd + 2),), torch.float32)
         pieces = workspace.get("attn_shared_pieces", (groups * row_blocks * nkv,), torch.int32)

@@ -7,31 +7,28 @@
 // A tile of 8 x 4 takes 12 reads of 16 bytes for 128 multiply-adds, which keeps the multiply-adds the bound and not shared memory.
 // What bounds the kernel: a page of head size 128 is 64 KB and takes an SM 1.5 us at the copy rate; its products take 16 rows
 // 1.1 us at the SM's full rate, 32 rows 2.1 us.  Pages come by TMA, keys in boxes of 32 dimensions and values in boxes of 32 keys,
-// whose 128-byte swizzle keeps the reads of neighbouring rows in different banks.
+// whose 128-byte swizzle keeps the reads of neighbouring rows in different banks.  Two blocks share an SM (one's barriers and
+// softmax under the other's products); the next page's keys are requested when the scores are done, its values after the products.
 //
 // Nothing is read before the wait for the kernels before: a page may have been copied by one of them.  Every wait on an mbarrier
 // is bounded; when a bound is hit the block records a code in tl_attn_shared_f32_error, waits (bounded) for its copies in flight and returns.
 #include "attention_shared.cuh"
 
-#define SF_THREADS 256          // that compute; a warp more brings the pages
+#define SF_THREADS 256
 #define SF_PLD (PAGE + 4)       // floats of a row of weights
 
 __device__ int tl_attn_shared_f32_error = 0;
 
-__device__ __forceinline__ void sf_bar() { asm volatile("bar.sync 1, 256;" ::: "memory"); }   // the computing warps
-
 template <int HD>
 struct SfSizes {
-  static constexpr int K = PAGE * HD * 4, V = HD * PAGE * 4, STAGE = K + V, STAGES = HD == 64 ? 4 : 2;
-  // stages, the shares of the keys of one unit's output (64 rows in all), queries of two units, weights, references and factors
-  static constexpr int smem(int rg) {
-    return STAGES * STAGE + 64 * HD * 4 + 8 * rg * (2 * HD + SF_PLD + 1) * 4 + SH_MAX_GROUPS * (int)sizeof(ShGroup) + 256;
-  }
+  static constexpr int K = PAGE * HD * 4, V = HD * PAGE * 4;
+  // a page's keys, a page's values (and the shares of the keys of a unit's output: 64 rows), queries, weights, factors, the groups
+  static constexpr int smem(int rg) { return K + V + 8 * rg * (HD + SF_PLD + 1) * 4 + SH_MAX_GROUPS * (int)sizeof(ShGroup) + 128; }
 };
 
 // RG: eights of rows that a unit holds: 1, 2 or 4.
 template <int HD, int RG>
-__global__ void __launch_bounds__(SF_THREADS + 32, 1)
+__global__ void __launch_bounds__(SF_THREADS, 2)
 attn_shared_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const ShArgs<float> a) {
   using Z = SfSizes<HD>;
   constexpr int ROWS = 8 * RG;
@@ -39,61 +36,78 @@ attn_shared_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   constexpr int DG = HD / 4, KV = SF_THREADS / (DG * RG);   // groups of dimensions; threads that share the keys of a tile of O
   static_assert(KV * ROWS == 64 * 128 / HD, "");
   extern __shared__ __align__(1024) uint8_t sf_smem[];
-  uint8_t* smem = sf_smem;
-  float* o_s = (float*)(smem + Z::STAGES * Z::STAGE);       // [KV][ROWS][HD] (head size 64: in two halves)
-  float* q_s = o_s + 64 * HD;                               // [2][ROWS][HD]
-  float* p_s = q_s + 2 * ROWS * HD;                         // [ROWS][SF_PLD]
+  uint8_t* kb = sf_smem;
+  uint8_t* vb = kb + Z::K;
+  float* o_s = (float*)vb;                                  // [KV][ROWS][HD] (head size 64: in two halves)
+  float* q_s = (float*)(vb + Z::V);                         // [ROWS][HD]
+  float* p_s = q_s + ROWS * HD;                             // [ROWS][SF_PLD]
   float* al_s = p_s + ROWS * SF_PLD;                        // [ROWS]
   ShGroup* table = (ShGroup*)(al_s + ROWS);
-  uint64_t* full_bar = (uint64_t*)(table + SH_MAX_GROUPS);
-  uint64_t* empty_bar = full_bar + Z::STAGES;
-  int* total_s = (int*)(empty_bar + Z::STAGES);             // [2]
-  volatile int* abort_flag = (volatile int*)(total_s + 2);
-  const int tid = threadIdx.x, warp = tid >> 5;
+  uint64_t* k_full = (uint64_t*)(table + SH_MAX_GROUPS);
+  uint64_t* v_full = k_full + 1;
+  int* total_s = (int*)(v_full + 1);                        // [3]
+  volatile int* abort_flag = (volatile int*)(total_s + 3);
+  const int tid = threadIdx.x;
   if (smem_u32(sf_smem) & 1023u) {         // swizzled tiles need that alignment
     if (tid == 0) atomicCAS(&tl_attn_shared_f32_error, 0, 9);
     return;
   }
   if (tid == 0) {
-    for (int s = 0; s < Z::STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], SF_THREADS / 32); }
+    mbar_init(k_full, 1);
+    mbar_init(v_full, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   pdl_wait();
   pdl_launch_dependents();
-  if (warp == SF_THREADS / 32) sh_make_line<1>(table, total_s, a, tid & 31);
+  if (tid < 32) sh_make_line<1>(table, total_s, a, gridDim.x, tid);
   __syncthreads();
-  const int total = total_s[0], share = sh_share(total_s, gridDim.x, a.parts);
+  const int total = total_s[0], gap = total_s[2], share = sh_share(total_s, gridDim.x, a.parts);
   const int t0 = min((int)blockIdx.x * share, total), t1 = min(t0 + share, total);
   const int G = a.nh / a.nkv;
   if (t0 >= t1) return;
 
-  if (warp == SF_THREADS / 32) {
-    if (!elect_one()) return;
-    bool ok = true;
-    int n = 0;
-    for (int t = t0; t < t1 && ok;) {
-      const ShPiece p = sh_locate<1>(table, a, t);
-      const int last = min(p.tiles, p.tile + t1 - t);
-      for (int j = p.tile; j < last; ++j, ++t, ++n) {
-        int owner, col;
-        sh_page(p, j, owner, col);
-        const int slab = a.page_table[(size_t)a.seq_slot[p.row0 + max(owner, 0)] * a.table_stride + col] * a.nkv + p.kvh;
-        const int s = n % Z::STAGES;
-        ok = tl_mbar_park(&empty_bar[s], ((uint32_t)(n / Z::STAGES) & 1u) ^ 1u, abort_flag, 1, &tl_attn_shared_f32_error);
-        if (!ok) break;
-        uint8_t* st = smem + (size_t)s * Z::STAGE;
-        mbar_expect_tx(&full_bar[s], Z::STAGE);
-#pragma unroll
-        for (int sub = 0; sub < HD / 32; ++sub) tma_load_2d(st + sub * (PAGE * 128), &tm_k, &full_bar[s], sub * 32, slab * PAGE);
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub) tma_load_2d(st + Z::K + sub * (HD * 128), &tm_v, &full_bar[s], sub * 32, slab * HD);
-      }
+  // One thread requests pages; it looks a page's place up a tile before it is wanted.
+  ShPiece ahead;
+  ahead.next = t0;
+  int ahead_j = 0;
+  bool more = false;               // `ahead` has another page
+  auto advance = [&] {             // to the next piece with tiles
+    do {
+      ahead = sh_locate(table, a, gap, ahead.next, t1);
+    } while (ahead.tile == ahead.last && ahead.next < t1);
+    ahead_j = ahead.tile;
+    more = ahead_j < ahead.last;
+  };
+  auto next_slab = [&]() -> int {
+    int owner, col;
+    sh_page(ahead, ahead_j, owner, col);
+    const int slab = a.page_table[(size_t)a.seq_slot[ahead.row0 + max(owner, 0)] * a.table_stride + col] * a.nkv + ahead.kvh;
+    if (++ahead_j == ahead.last) {
+      more = false;
+      if (ahead.next < t1) advance();
     }
-    if (!ok)             // given up: what is in flight lands before the block ends, or for as long as a wait may take
-      for (int i = max(0, n - Z::STAGES); i < n; ++i)
-        for (uint32_t k = 0; k < TL_WAIT_LIMIT / 64 && !tl_mbar_try_wait(&full_bar[i % Z::STAGES], (uint32_t)(i / Z::STAGES) & 1u); ++k) {}
-    return;
+    return slab;
+  };
+  auto issue_k = [&](int slab) {
+    mbar_expect_tx(k_full, Z::K);
+#pragma unroll
+    for (int sub = 0; sub < HD / 32; ++sub) tma_load_2d(kb + sub * (PAGE * 128), &tm_k, k_full, sub * 32, slab * PAGE);
+  };
+  auto issue_v = [&](int slab) {
+    mbar_expect_tx(v_full, Z::V);
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) tma_load_2d(vb + sub * (HD * 128), &tm_v, v_full, sub * 32, slab * HD);
+  };
+  int slab = 0;
+  bool pending = false;            // `slab` is that of a page that has not been requested
+  if (tid == 0) {
+    advance();
+    if (more) {
+      slab = next_slab();
+      issue_k(slab);
+      issue_v(slab);
+    }
   }
 
   // scores: this thread's share of the dimensions, its keys kg + 16 i, its rows 8 rs + j.  Where four threads share the
@@ -105,37 +119,37 @@ attn_shared_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   const int sr = tid / TR, sk = tid % TR;
   // output: dimensions dg + DG i, keys of share kv, rows 8 ro + j
   const int dg = tid % DG, kv = (tid / DG) % KV, ro = tid / (DG * KV);
-  auto load_q = [&](const ShPiece& p, int buf) {
-    for (int i = tid; i < ROWS * DG; i += SF_THREADS) {
-      const int r = i / DG, c = i % DG;
-      reinterpret_cast<float4*>(q_s + buf * ROWS * HD)[i] =
-          r < p.beams * G ? reinterpret_cast<const float4*>(a.q + ((size_t)(p.row0 + r / G) * a.nh + p.kvh * G + r % G) * HD)[c]
+  const ShRow row_of(tid / DG, G), soft_row(sr, G), out_row(tid / HD, G);
+  auto load_q = [&](const ShPiece& p) {
+    ShRow at = row_of;
+#pragma unroll 1
+    for (int r = tid / DG; r < ROWS; r += SF_THREADS / DG) {
+      reinterpret_cast<float4*>(q_s)[r * DG + dg] =
+          r < p.beams * G ? reinterpret_cast<const float4*>(a.q + ((size_t)(p.row0 + at.beam) * a.nh + p.kvh * G + at.head) * HD)[dg]
                           : make_float4(0.f, 0.f, 0.f, 0.f);
+      at.step(SF_THREADS / DG);
     }
   };
   // A wait that runs out leaves the loop's barriers in place: the warps go through them to the end (every later wait returns at
   // once), and what they write is not valid.
-  int n = 0, unit = 0;
-  ShPiece p = sh_locate<1>(table, a, t0);
-  load_q(p, 0);
-  for (int t = t0; t < t1; ++unit) {
-    const int last = min(p.tiles, p.tile + t1 - t), R = p.beams * G, next = t + last - p.tile;
-    ShPiece np = p;
-    if (next < t1) {
-      np = sh_locate<1>(table, a, next);
-      load_q(np, (unit + 1) & 1);
-    }
-    const float* qq_s = q_s + (unit & 1) * ROWS * HD;
+  int n = 0;
+  for (int t = t0; t < t1;) {
+    const ShPiece p = sh_locate(table, a, gap, t, t1);
+    const int last = p.last, R = p.beams * G;
+    t = p.next;
+    if (p.tile == last) continue;
+    load_q(p);
     float m = -INFINITY, l = 0.0f;           // of row sr, the sum of this thread's keys
     float acc[8][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-    sf_bar();                                // the queries are there, the unit before has left shared memory
+    __syncthreads();                         // the queries are there
     for (int i = p.tile; i < last; ++i, ++n) {
-      const int s = n % Z::STAGES;
-      tl_mbar_wait(&full_bar[s], (uint32_t)(n / Z::STAGES) & 1u, abort_flag, 2, &tl_attn_shared_f32_error);
-      const uint8_t* kb = smem + (size_t)s * Z::STAGE;
-      const uint8_t* vb = kb + Z::K;
+      if (tid == 0) {
+        pending = more;
+        if (more) slab = next_slab();
+      }
+      tl_mbar_park(k_full, (uint32_t)n & 1u, abort_flag, 1, &tl_attn_shared_f32_error);
       int owner, col;
       sh_page(p, i, owner, col);
       const int key0 = col * PAGE, r0 = owner > 0 ? owner * G : 0, r1 = owner >= 0 ? r0 + G : R;   // the rows that see the page
@@ -153,16 +167,18 @@ attn_shared_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
             const int row = kg + 16 * e;
             kk[e] = *reinterpret_cast<const float4*>(kb + (chunk >> 3) * (PAGE * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
           }
+          float4 qq[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) qq[j] = reinterpret_cast<const float4*>(q_s + (8 * rs + j) * HD)[chunk];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float4 qq = reinterpret_cast<const float4*>(qq_s + (8 * rs + j) * HD)[chunk];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float& v = sc[4 * j + e];
-              v = fmaf(qq.x, kk[e].x, v);
-              v = fmaf(qq.y, kk[e].y, v);
-              v = fmaf(qq.z, kk[e].z, v);
-              v = fmaf(qq.w, kk[e].w, v);
+              v = fmaf(qq[j].x, kk[e].x, v);
+              v = fmaf(qq[j].y, kk[e].y, v);
+              v = fmaf(qq[j].z, kk[e].z, v);
+              v = fmaf(qq[j].w, kk[e].w, v);
             }
           }
         }
@@ -187,7 +203,8 @@ attn_shared_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           p_s[(8 * rs + (id >> 2)) * SF_PLD + kg + 16 * (id & 3)] = sc[j];
         }
       }
-      sf_bar();
+      __syncthreads();
+      if (tid == 0 && pending) issue_k(slab);
       {
         const bool in = sr >= r0 && sr < r1;
         float v[2 * RG], mx = m;
@@ -210,7 +227,8 @@ attn_shared_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         m = mx;
         if (sk == 0) al_s[sr] = alpha;
       }
-      sf_bar();
+      tl_mbar_park(v_full, (uint32_t)n & 1u, abort_flag, 2, &tl_attn_shared_f32_error);
+      __syncthreads();
       if (8 * ro < r1 && 8 * ro + 8 > r0) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -237,23 +255,30 @@ attn_shared_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
               if (at + 3 < p.lo || at + 3 >= p.len) vv[e].w = 0.0f;
             }
           }
+          float4 pp[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            // (a row that does not see the page stays as it is, whatever the values are)
-            if (owner >= 0 && (8 * ro + j < r0 || 8 * ro + j >= r1)) continue;
-            const float4 pp = *reinterpret_cast<const float4*>(p_s + (8 * ro + j) * SF_PLD + 4 * chunk);
+          for (int j = 0; j < 8; ++j) pp[j] = *reinterpret_cast<const float4*>(p_s + (8 * ro + j) * SF_PLD + 4 * chunk);
+          auto row = [&](int j) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              acc[j][e] = fmaf(pp.x, vv[e].x, acc[j][e]);
-              acc[j][e] = fmaf(pp.y, vv[e].y, acc[j][e]);
-              acc[j][e] = fmaf(pp.z, vv[e].z, acc[j][e]);
-              acc[j][e] = fmaf(pp.w, vv[e].w, acc[j][e]);
+              acc[j][e] = fmaf(pp[j].x, vv[e].x, acc[j][e]);
+              acc[j][e] = fmaf(pp[j].y, vv[e].y, acc[j][e]);
+              acc[j][e] = fmaf(pp[j].z, vv[e].z, acc[j][e]);
+              acc[j][e] = fmaf(pp[j].w, vv[e].w, acc[j][e]);
             }
+          };
+          if (owner < 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) row(j);
+          } else {                 // a row that does not see the page stays as it is, whatever the values are
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (8 * ro + j >= r0 && 8 * ro + j < r1) row(j);
           }
         }
       }
-      sf_bar();                  // the page and its weights are used up
-      if ((tid & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty_bar[s])) : "memory");
+      __syncthreads();           // the page and its weights are used up
+      if (tid == 0 && i + 1 < last) issue_v(slab);
     }
     // ---- the unit's end: the shares of the keys
     const int first_block = p.start / share, pieces = (p.start + p.tiles - 1) / share - first_block + 1;
@@ -261,9 +286,13 @@ attn_shared_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     if (tid == 0 && slot == 0) a.unit_parts[p.unit] = pieces;
 #pragma unroll
     for (int d = TR / 2; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-    auto head_of = [&](int r) { return (size_t)(p.row0 + r / G) * a.nh + p.kvh * G + r % G; };
+    // (What runs once per unit is fetched from afar, some ten cycles an instruction: it is written as loops, without divisions.)
+    const int heads = a.parts * (HD + 2);
+    auto part_of = [&](const ShRow& at) {
+      return a.part + ((size_t)(p.row0 + at.beam) * a.nh + p.kvh * G + at.head) * heads + slot * (HD + 2);
+    };
     if (sk == 0 && sr < R) {
-      float* dst = a.part + (head_of(sr) * a.parts + slot) * (HD + 2) + HD;
+      float* dst = part_of(soft_row) + HD;
       dst[0] = m;
       dst[1] = l;
     }
@@ -271,34 +300,42 @@ attn_shared_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 #pragma unroll
     for (int h = HALVES - 1; h >= 0; --h) {
       if (kv / (KV / HALVES) == h) {
+        float* o = o_s + ((kv % (KV / HALVES)) * ROWS + 8 * ro) * HD + dg;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float* o = o_s + ((kv % (KV / HALVES)) * ROWS + 8 * ro + j) * HD + dg + DG * e;
-            *o = h == HALVES - 1 ? acc[j][e] : *o + acc[j][e];
-          }
+          for (int e = 0; e < 4; ++e) o[j * HD + DG * e] = h == HALVES - 1 ? acc[j][e] : o[j * HD + DG * e] + acc[j][e];
       }
-      sf_bar();
+      __syncthreads();
     }
-    for (int i = tid; i < R * HD; i += SF_THREADS) {
+    ShRow at = out_row;
+#pragma unroll 1
+    for (int r = tid / HD; r < R; r += SF_THREADS / HD) {
       float o = 0.0f;
 #pragma unroll
-      for (int k = 0; k < KV / HALVES; ++k) o += o_s[k * ROWS * HD + i];
-      a.part[(head_of(i / HD) * a.parts + slot) * (HD + 2) + i % HD] = o;
+      for (int k = 0; k < KV / HALVES; ++k) o += o_s[(k * ROWS + r) * HD + tid % HD];
+      part_of(at)[tid % HD] = o;
+      at.step(SF_THREADS / HD);
     }
-    t = next;
-    p = np;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the next values come where the shares lay
+    __syncthreads();
+    if (tid == 0 && pending) issue_v(slab);
   }
+  // (if a wait ran out: what is in flight lands before the block ends, or for as long as a wait may take)
+  if (*abort_flag && tid == 0) {
+    const uint32_t parity = (uint32_t)(n - 1) & 1u;
+    for (uint32_t k = 0; k < TL_WAIT_LIMIT / 64 && !(tl_mbar_try_wait(k_full, parity) && tl_mbar_try_wait(v_full, parity)); ++k) {}
+  }
+  __syncthreads();
 }
 
 template <int HD, int RG>
 static int sf_launch(const CUtensorMap& tk, const CUtensorMap& tv, const ShArgs<float>& a, int blocks, cudaStream_t stream) {
   constexpr int smem = SfSizes<HD>::smem(RG);
-  static_assert(smem <= 232448, "a block's shared memory");
+  static_assert(smem <= 115 * 1024, "a block's shared memory");
   const cudaError_t set = tl_allow_smem<attn_shared_f32_kernel<HD, RG>>(smem);
   if (set != cudaSuccess) return (int)set;
-  return tl_launch(attn_shared_f32_kernel<HD, RG>, dim3(blocks), dim3(SF_THREADS + 32), (size_t)smem, stream, tk, tv, a);
+  return tl_launch(attn_shared_f32_kernel<HD, RG>, dim3(blocks), dim3(SF_THREADS), (size_t)smem, stream, tk, tv, a);
 }
 template <int HD>
 static int sf_run(const void* k_pages, const void* v_pages, long long n_pages, const ShArgs<float>& a, int blocks, int group_rows,
