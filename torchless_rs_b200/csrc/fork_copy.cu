@@ -2,16 +2,22 @@
 // part of a page into a page that the sequence may write to.  (The reference has one sequence and never copies its cache,
 // src/model/kv_cache.rs:23-53.)
 //
-// Nothing is computed: the bound is the memory's copy rate, twice the bytes that move.  A block moves up to 16 KB (slots)
-// or one head's part of one layer's page (pages); a thread has four 16-byte loads in flight before its first store.  The
-// pairs travel as kernel arguments, so that nothing has to be brought to the device first.  Sources are never
-// destinations (the caller's rule, checked there), so blocks may run in any order.  The next kernel is not let go early: attention
-// kernels read pages that "earlier steps" have filled before they wait, and a copied page is one of those.
+// Nothing is computed: the bound is the memory's copy rate, twice the bytes that move.  A block moves up to 16 KB of a slot, or one head's
+// keys or values of one layer's page; a thread has four 16-byte loads in flight before its first store (two and two where
+// values end inside a sector: with one or three and three of them the copy below takes 60 and 56 us).  The pairs travel as kernel
+// arguments, so that nothing has to be brought to the device first.  Sources are never destinations (the caller's rule, checked there), so
+// blocks may run in any order.  The next kernel is not let go early: attention kernels read pages that "earlier steps" have filled before they
+// wait, and a copied page is one of those.
+//
+// Measured: 32 layers x 24 pages, 8 heads of 128 in bfloat16: whole pages 62 us (6.5 TB/s read and written); 1 to 63 positions, 32 in the
+// mean, 56 us (3.4 TB/s of what is asked for: keys go at 6.1, but a part of a value row of 128 bytes costs whole 64-byte units of
+// memory, read and written); half the keys alone 32 us.
 #include "common.cuh"
 
 #define FORK_PAIRS 256
 #define FORK_THREADS 256
 #define FORK_AHEAD 4
+#define FORK_BLEND 2
 
 struct ForkPairs {
   int src[FORK_PAIRS];
@@ -41,17 +47,19 @@ TL_NAME(copy_slots_kernel)(unsigned char* __restrict__ storage, const __grid_con
 
 // One layer's key pages [pages][heads][TL_PAGE][dim] and after them its value pages [pages][heads][vdim][TL_PAGE] (vdim 0: none):
 // of a head, the first `count` positions.  Those are the first count * dim numbers of its keys, and the first `count` numbers
-// of every row of its values; what lies beyond is not written.
+// of every row of its values; what lies beyond is not written.  A block copies a head's keys (blockIdx.x < heads) or its values.
 template <typename T>
 __global__ void __launch_bounds__(FORK_THREADS)
 TL_NAME(copy_pages_kernel)(T* __restrict__ storage, const __grid_constant__ ForkPairs p, long long layer_elems, long long v_off,
                            int heads, int dim, int vdim) {
   constexpr int W = 16 / sizeof(T);                 // numbers in 16 bytes
   pdl_wait();
-  const int head = blockIdx.x, c = p.count[blockIdx.y], tid = threadIdx.x;
+  const int bx = blockIdx.x;
+  const bool values = bx >= heads;
+  const int head = values ? bx - heads : bx, c = p.count[blockIdx.y], tid = threadIdx.x;
   T* layer = storage + (size_t)blockIdx.z * layer_elems;
   const size_t from = (size_t)p.src[blockIdx.y] * heads + head, to = (size_t)p.dst[blockIdx.y] * heads + head;
-  {
+  if (!values) {
     const T* src = layer + from * TL_PAGE * dim;
     T* dst = layer + to * TL_PAGE * dim;
     const int n = c * dim / W;
@@ -65,31 +73,40 @@ TL_NAME(copy_pages_kernel)(T* __restrict__ storage, const __grid_constant__ Fork
         if (i0 + k * FORK_THREADS < n) __stcs(reinterpret_cast<uint4*>(dst) + i0 + k * FORK_THREADS, v[k]);
     }
     for (int i = n * W + tid; i < c * dim; i += FORK_THREADS) dst[i] = src[i];   // a key of no multiple of 16 bytes
+    return;
   }
-  if (vdim == 0) return;
   const T* src = layer + v_off + from * vdim * TL_PAGE;
   T* dst = layer + v_off + to * vdim * TL_PAGE;
-  const int per = (c + W - 1) / W, n = vdim * per;  // 16-byte pieces of a row that hold a copied position
-  for (int i0 = tid; i0 < n; i0 += FORK_THREADS * FORK_AHEAD) {
-    uint4 v[FORK_AHEAD];
-    int at[FORK_AHEAD], left[FORK_AHEAD];
+  // 16-byte pieces of a row up to the end of the 32-byte sector in which the copied positions end.  That sector is read from the
+  // destination too and written whole: memory takes whole sectors, and one written in part is fetched by the cache first, at
+  // half the rate (the copy above with 17 positions each: 62 us written in part, 48 so).
+  const int per = (c + 2 * W - 1) / (2 * W) * 2, n = vdim * per;
+  const float inv = 1.f / per;
+  for (int i0 = tid; i0 < n; i0 += FORK_THREADS * FORK_BLEND) {
+    uint4 v[FORK_BLEND], w[FORK_BLEND];
+    int at[FORK_BLEND], left[FORK_BLEND];
 #pragma unroll
-    for (int k = 0; k < FORK_AHEAD; ++k) {
-      const int i = i0 + k * FORK_THREADS, row = i / per, piece = i - row * per;
+    for (int k = 0; k < FORK_BLEND; ++k) {
+      // i / per by a product: i + 1/2 is at least 1 / (2 per) >= 1/32 away from the next whole row, and with rows below 2^16 the two
+      // roundings move the result by less than 2^16 * 2^-22 = 1/64
+      const int i = i0 + k * FORK_THREADS, row = (int)((i + 0.5f) * inv), piece = i - row * per;
       at[k] = row * TL_PAGE + piece * W;
-      left[k] = i < n ? c - piece * W : 0;
-      if (i < n) v[k] = __ldcs(reinterpret_cast<const uint4*>(src + at[k]));
+      left[k] = i < n ? c - piece * W : W + 1;      // (W + 1: nothing to read or write)
+      if (i < n && left[k] > 0) v[k] = __ldcs(reinterpret_cast<const uint4*>(src + at[k]));
+      if (left[k] < W) w[k] = __ldcs(reinterpret_cast<const uint4*>(dst + at[k]));
     }
 #pragma unroll
-    for (int k = 0; k < FORK_AHEAD; ++k) {
-      if (left[k] >= W) {
-        __stcs(reinterpret_cast<uint4*>(dst + at[k]), v[k]);
-      } else if (left[k] > 0) {                     // the piece in which the copied positions end
+    for (int k = 0; k < FORK_BLEND; ++k) {
+      if (i0 + k * FORK_THREADS >= n) break;
+      if (left[k] < W) {
         const T* e = reinterpret_cast<const T*>(&v[k]);
+        T* f = reinterpret_cast<T*>(&w[k]);
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j)
-          if (j < left[k]) dst[at[k] + j] = e[j];
+        for (int j = 0; j < W; ++j)
+          if (j < left[k]) f[j] = e[j];
+        v[k] = w[k];
       }
+      __stcs(reinterpret_cast<uint4*>(dst + at[k]), v[k]);
     }
   }
 }
@@ -135,7 +152,7 @@ extern "C" int TL_NAME(tl_copy_pages)(void* storage, int layers, long long layer
                                       int vdim, const int* src, const int* dst, const int* count, int n,
                                       cudaStream_t stream) {
   if (n <= 0 || layers <= 0) return 0;
-  if (heads <= 0 || dim <= 0 || vdim < 0 || pages <= 0 || ((uintptr_t)storage & 15) ||
+  if (heads <= 0 || heads > 65536 || dim <= 0 || vdim < 0 || pages <= 0 || ((uintptr_t)storage & 15) ||
       layer_elems < (long long)pages * heads * TL_PAGE * (dim + vdim))
     return TL_ERR_BAD_ARG;
   if (layers > 65535 || dim > 65536 || vdim > 65536 || (layer_elems * (long long)sizeof(act_t)) % 16) return TL_ERR_UNSUPPORTED;
@@ -147,7 +164,7 @@ extern "C" int TL_NAME(tl_copy_pages)(void* storage, int layers, long long layer
     const int m = n - i0 < FORK_PAIRS ? n - i0 : FORK_PAIRS;
     ForkPairs p;
     TL_NAME(fork_pairs)(p, src + i0, dst + i0, count + i0, m);
-    const int st = tl_launch(TL_NAME(copy_pages_kernel)<act_t>, dim3(heads, m, layers), dim3(FORK_THREADS), 0, stream,
+    const int st = tl_launch(TL_NAME(copy_pages_kernel)<act_t>, dim3(vdim ? 2 * heads : heads, m, layers), dim3(FORK_THREADS), 0, stream,
                              (act_t*)storage, p, layer_elems, v_off, heads, dim, vdim);
     if (st) return st;
   }
