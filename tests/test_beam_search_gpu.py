@@ -17,13 +17,19 @@ import rupasun_tiny
 import tovapel_tiny
 from helpers_gpu import TinyModel, assert_close
 from tiny import CONFIGS, make_model_dir, random_tokens, read_weights_numpy
-from torchless_rs_b200.csrc import ops
+from torchless_rs_b200.csrc import attention_shared, ops
 
 pytestmark = pytest.mark.gpu
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 DESIGNS = {"kikopel": (kikopel_tiny.KModel, "P"), "dunesun": (dunesun_tiny.DModel, "A"), "tovapel": (tovapel_tiny.TModel, "P"),
            "rupasun": (rupasun_tiny.TModel, "P"), "fezolorn": (fezolorn_tiny.FModel, None), "beralix": (beralix_tiny.BModel, None)}
+
+
+@pytest.fixture(autouse=True)
+def shared_pages_are_read_together(monkeypatch):
+    """These models are far too small for it to pay."""
+    monkeypatch.setattr(attention_shared, "WORTH", {t: (0.0, 0.0) for t in attention_shared.WORTH})
 
 
 def _design(name, dtype):
@@ -145,6 +151,24 @@ def test_the_grouped_mixers_of_other_designs_take_shared_pages():
     assert ops.launch_counts().get("attn_shared", 0) > before
     rms = np.sqrt(((outs[0] - outs[1]) ** 2).mean()) / np.sqrt((outs[0] ** 2).mean())
     assert rms <= 2e-2           # the bound of that design's tests
+
+
+def test_few_shared_keys_are_read_row_by_row(monkeypatch):
+    monkeypatch.undo()
+    tm = TinyModel("D", "bfloat16", seed=6, max_tokens=1024)
+    eng = tm.engine
+    slots = eng.start_sequences(2)
+    eng.step(slots[:1], [random_tokens(np.random.default_rng(0), 130, eng.vocab_size)])
+    eng.fork([slots[0]], [slots[1]])
+    before = ops.launch_counts().get("attn_shared", 0)
+    shared = eng.step(slots, [[1], [2]], groups=[2]).clone()
+    assert ops.launch_counts().get("attn_shared", 0) == before
+    eng.end_sequences(slots)
+    slots = eng.start_sequences(2)
+    eng.step(slots[:1], [random_tokens(np.random.default_rng(0), 130, eng.vocab_size)])
+    eng.fork([slots[0]], [slots[1]])
+    assert torch.equal(eng.step(slots, [[1], [2]]), shared)
+    eng.end_sequences(slots)
 
 
 def _plain_search(tm, prompt, max_tokens, beams, penalty, stop):

@@ -21,9 +21,7 @@ static_assert(PAGE == 64, "the tiles are laid out for pages of 64 tokens");
 
 #define SH_MAX_PARTS 160
 #define SH_MAX_GROUPS 256
-#ifndef SH_UNIT_TILES
 #define SH_UNIT_TILES 4
-#endif
 
 template <typename T>
 struct ShArgs {

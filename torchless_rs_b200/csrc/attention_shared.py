@@ -19,6 +19,14 @@ BLOCK_ROWS = {torch.bfloat16: 64, torch.float32: 32}    # rows of a unit (rows o
 TILE_PAGES = {torch.bfloat16: 2, torch.float32: 1}      # pages that a block takes at a time
 PER_SM = {torch.bfloat16: 1, torch.float32: 2}          # resident blocks
 MAX_PARTS = 160                # pieces of a unit that the merge takes
+# When shared pages are worth the kernel: (bytes, share).  It takes some 4 us more than the per-row kernels (two launches, units whose tiles
+# differ, one block for all beams' own pages), which read what rows share from the L2 cache at up to 9 TB/s; so the bytes of keys and values
+# that rows need not read again have to exceed `bytes` and `share` of those that rows hold alone.  Measured over 1296 shapes (1 to 16
+# groups of 2 to 8 rows, 64 to 4096 common and 20 to 1000 own tokens, six head layouts, cold cache), per row / shared: bfloat16, 32 over
+# 8 heads of 128, 4 groups of 4: 256 + 200 tokens 10.7 / 13.4 us, 1024 + 20 14.6 / 13.4, 4096 + 20 38 / 17; 16 groups of 8 with 4096 +
+# 20 238 / 64; 32-bit, 1 group of 8, 256 + 20 14 / 17, 1024 + 20 31 / 23.  The rule is 0.5 % (bfloat16) and 4 % (32-bit) above the better of both in
+# the geometric mean; always per row 11 % and 48 %, always shared 37 % and 6 %.
+WORTH = {torch.bfloat16: (60e6, 0.5), torch.float32: (16e6, 0.0)}
 
 for _hd in HEAD_DIMS:
     build.register_library(f"attn_shared_bf16_hd{_hd}", ("attention_shared.cu",), (f"-DHEAD_DIM={_hd}",))
@@ -45,6 +53,20 @@ def shared_plan(lens: Tuple[int, ...], shared: Tuple[int, ...], group_rows: int,
         longest = max(longest, tiles, -(-(max(bound, border - first) + (end - border) * beams) // tile) if bound else 0)
     share = max(1, -(-total // blocks))
     return row_blocks, max(2, min(MAX_PARTS, -(-longest // share) + 3))
+
+
+def worth_sharing(rows: Sequence[int], lens: Sequence[int], shared: Sequence[int], nkv: int, head_dim: int,
+                  window: Optional[int], dtype: torch.dtype) -> bool:
+    """Whether reading common pages once saves more than the kernel costs; per group its rows, length and common pages."""
+    saved = own = 0
+    for b, n, c in zip(rows, lens, shared):
+        first = max(0, n - window) if window else 0
+        border = min(max(c * PAGE, first), n)
+        saved += (b - 1) * (border - first)
+        own += b * (n - border)
+    token = 2 * nkv * head_dim * dtype.itemsize
+    least, share = WORTH[dtype]
+    return saved * token > least + share * own * token
 
 
 _sms: Dict[int, int] = {}
@@ -147,13 +169,17 @@ class SharedAttention:
 
 
 def run_shared(q, cache_view, out, batch, nh: int, nkv: int, window, scale: float, workspace) -> bool:
-    """A decode step whose rows hold leading pages together (`batch.groups`).  False where no kernel takes it: the caller
-    then uses one that reads every row's pages for itself."""
-    kernel = SharedAttention.get(q.dtype, q.shape[1] // nh)
-    if kernel is None or not kernel.takes(nh, nkv):
+    """A decode step whose rows hold leading pages together (`batch.groups`).  False where no kernel takes it or too little is shared:
+    the caller then uses one that reads every row's pages for itself.  (A recorded step keeps what it was recorded with: steps of one
+    graph have lengths in one bucket, and either kernel is right for all of them.)"""
+    g, c, hd = batch.groups, cache_view, q.shape[1] // nh
+    kernel = SharedAttention.get(q.dtype, hd)
+    if kernel is None or not kernel.takes(nh, nkv) or len(g.rows) > MAX_GROUPS:
         return False
-    g, c = batch.groups, cache_view
-    if len(g.rows) > MAX_GROUPS:
+    key = ("attn_shared", nkv, hd, window, q.dtype)
+    if key not in batch.plans:
+        batch.plans[key] = worth_sharing(g.rows, g.lens, g.shared, nkv, hd, window, q.dtype)
+    if not batch.plans[key]:
         return False
     seen = min(batch.len_bucket, window + PAGE) if window else batch.len_bucket
     kernel.decode(q, c.k_pages, c.v_pages, out, batch.seq_len, batch.seq_slot, c.page_table, g.start, g.pages, nh, nkv, window, scale,

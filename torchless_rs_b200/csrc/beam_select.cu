@@ -83,12 +83,8 @@ struct BsPart {
 };
 
 #define BS_TILE (BS_THREADS * 16)
-#ifndef BS_MAX_TILES
 #define BS_MAX_TILES 32
-#endif
-#ifndef BS_PER_SM
 #define BS_PER_SM 4                // resident blocks
-#endif
 
 // GS threads form a group (256 / GS >= 2 n groups, or as many as there are threads).
 template <int GS>
