@@ -574,7 +574,7 @@ extern "C" int FN(tl_attn_shared)(const void* q, const void* k_pages, const void
                     table_stride, groups, nh, nkv, window, scale * 1.4426950408889634f, parts, row_blocks, beams};
   const int st = R <= 16 ? sh_run<16>(tk, tv, a, blocks, stream) : R <= 32 ? sh_run<32>(tk, tv, a, blocks, stream) : sh_run<64>(tk, tv, a, blocks, stream);
   if (st) return st;
-  return tl_launch(attn_shared_merge_kernel<HEAD_DIM, true, true, __nv_bfloat16>, dim3(nh, group_rows, groups), dim3(HEAD_DIM), 0, stream, a,
+  return tl_launch(attn_shared_merge_kernel<HEAD_DIM, true, true, __nv_bfloat16>, dim3((nh * (HEAD_DIM / 64) + 3) / 4, group_rows, groups), dim3(SH_MERGE_THREADS), 0, stream, a,
                    (const __nv_bfloat16*)k_pages, (const __nv_bfloat16*)v_pages);
 }
 

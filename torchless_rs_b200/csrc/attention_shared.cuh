@@ -10,10 +10,6 @@
 #include "per_device.cuh"
 #include "umma.cuh"
 
-#include <map>
-#include <mutex>
-#include <tuple>
-
 #ifndef PAGE
 #define PAGE TL_PAGE
 #endif
@@ -21,6 +17,8 @@ static_assert(PAGE == 64, "the tiles are laid out for pages of 64 tokens");
 
 #define SH_MAX_PARTS 160
 #define SH_MAX_GROUPS 256
+#define SH_PART_TAIL 2                 // floats behind a piece's weighted sum: its reference and sum
+#define SH_MERGE_THREADS 128
 #define SH_UNIT_TILES 4
 
 template <typename T>
@@ -84,7 +82,7 @@ __device__ __forceinline__ void sh_make_line(ShGroup* table, int* totals, const 
     int n = 0, u = 0;
     if (g < a.groups) {
       e.row0 = a.group_start[g];
-      const int rows = a.group_start[g + 1] - e.row0;
+      const int rows = min(a.group_start[g + 1] - e.row0, a.beams * a.row_blocks);
       if (rows > 0) {
         const ShSpan s = sh_span(a.seq_len[e.row0], a.window, a.group_pages[g]);
         e.len = s.len; e.lo = s.lo; e.first = s.first; e.common = s.common; e.own = s.own;
@@ -173,102 +171,129 @@ __device__ __forceinline__ void sh_page(const ShPiece& p, int i, int& owner, int
   }
 }
 
-// Merges the pieces of one (row, head), a thread per dimension, in the order of the keys.  A row without any key (of length 0) gives zero.  EXP2: the maxima are logarithms to the base 2.
+// Merges the pieces of (row, head) pairs in the order of the keys, 64 of a head's numbers a warp, two a lane.  A row without any key (of
+// length 0) gives zero.  EXP2: the references are logarithms to the base 2.  (Little code and no barriers: this runs when everything
+// else is done, so that each step of it is waited for.  A block per pair with a thread per number took 1 us more at 8 prompts x 4 beams of the
+// 7B sizes and 2 us more in 32-bit.)
 //
 // AGAIN: a result that is no number is computed again from the keys that the row sees, one page after the other (the first kernel
 // multiplies values that it does not see by zero).  That is slow, and needed only where the cache holds values that are no numbers.
 template <int HD, bool EXP2, bool AGAIN, typename T>
-__global__ void __launch_bounds__(HD)
+__global__ void __launch_bounds__(SH_MERGE_THREADS)
 attn_shared_merge_kernel(const ShArgs<T> a, const T* __restrict__ k_pages, const T* __restrict__ v_pages) {
-  __shared__ float f_s[SH_MAX_PARTS];
+  constexpr int E = 2, SPLIT = HD / 64, AHEAD = 24, STRIDE = HD + SH_PART_TAIL;
   // what the call was given may be read before the wait: the kernel before this one has waited for those that wrote it
-  const int h = blockIdx.x, in_group = blockIdx.y, g = blockIdx.z, d = threadIdx.x, lane = d & 31;
+  const int lane = threadIdx.x & 31, w = blockIdx.x * (SH_MERGE_THREADS / 32) + (threadIdx.x >> 5);
+  const int h = w / SPLIT, d0 = w % SPLIT * 64 + E * lane, in_group = blockIdx.y, g = blockIdx.z;
   const int row0 = a.group_start[g], row = row0 + in_group;
-  const bool there = row < a.group_start[g + 1];
+  const bool there = row < a.group_start[g + 1] && h < a.nh;
   const ShSpan span = sh_span(there ? a.seq_len[row0] : 0, a.window, a.group_pages[g]);
+  const int kvh = h / (a.nh / a.nkv);
   pdl_wait();
   pdl_launch_dependents();
   if (!there) return;
   const size_t head = (size_t)row * a.nh + h;
-  auto store = [&](float v) {
-    if constexpr (sizeof(T) == 2) a.out[head * HD + d] = __float2bfloat16_rn(v); else a.out[head * HD + d] = v;
+  float acc[E] = {}, l = 0.0f, m = -INFINITY;
+  auto store = [&](float by) {
+    T* dst = a.out + head * HD + d0;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<__nv_bfloat162*>(dst + e) = __floats2bfloat162_rn(acc[e] / by, acc[e + 1] / by);
+      else
+        *reinterpret_cast<float2*>(dst + e) = make_float2(acc[e] / by, acc[e + 1] / by);
+    }
   };
   if (span.common + span.own == 0) {
-    store(0.0f);
+    store(1.0f);
     return;
   }
-  const float* src = a.part + head * a.parts * (HD + 2);
-  constexpr int AHEAD = 8;         // of the first pieces this thread's number is fetched before it is known how many there are
-  float v[AHEAD];
+  const float* src = a.part + head * a.parts * STRIDE;
+  float v[AHEAD][E];
+  auto fetch = [&](int s0) {
 #pragma unroll
-  for (int s = 0; s < AHEAD; ++s) v[s] = s < a.parts ? src[s * (HD + 2) + d] : 0.0f;
-  const int kvh = h / (a.nh / a.nkv), parts = a.unit_parts[((size_t)g * a.row_blocks + in_group / a.beams) * a.nkv + kvh];
-  // every warp: the largest reference, the factors, the sum (a piece in which this row sees no key has a reference of -inf)
-  constexpr int ROUNDS = (SH_MAX_PARTS + 31) / 32;
-  float ref[ROUNDS], sum[ROUNDS], m = -INFINITY, l = 0.0f;
+    for (int k = 0; k < AHEAD; ++k)
 #pragma unroll
-  for (int i = 0; i < ROUNDS; ++i) {
-    ref[i] = -INFINITY;
-    sum[i] = 0.0f;
-    if (32 * i >= parts) continue;       // (few pieces: little of this is fetched and run)
-    const int s = lane + 32 * i;
-    ref[i] = s < parts ? src[s * (HD + 2) + HD] : -INFINITY;
-    sum[i] = s < parts ? src[s * (HD + 2) + HD + 1] : 0.0f;
-    m = fmaxf(m, ref[i]);
+      for (int e = 0; e < E; e += 2) {
+        const float2 x = s0 + k < a.parts ? *reinterpret_cast<const float2*>(src + (s0 + k) * STRIDE + d0 + e) : make_float2(0.0f, 0.0f);
+        v[k][e] = x.x; v[k][e + 1] = x.y;
+      }
+  };
+  fetch(0);                        // the first pieces' numbers, before it is known how many there are
+  const int parts = a.unit_parts[((size_t)g * a.row_blocks + in_group / a.beams) * a.nkv + kvh];
+  for (int s0 = 0; s0 < parts; s0 += 32) {
+    // references and sums of 32 pieces (a piece in which this row sees no key has a reference of -inf)
+    const float2 rs = s0 + lane < parts ? *reinterpret_cast<const float2*>(src + (s0 + lane) * STRIDE + HD) : make_float2(-INFINITY, 0.0f);
+    float top = fmaxf(m, rs.x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    auto weight = [&](float ref) { return ref == -INFINITY ? 0.0f : EXP2 ? exp2f(ref - top) : expf(ref - top); };
+    const float f = weight(rs.x), old = weight(m);
+    float sum = f * rs.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    l = l * old + sum;
+    m = top;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= old;
+    const int end = min(s0 + 32, parts);
+    for (int s = s0; s < end; s += AHEAD) {
+      if (s > 0) fetch(s);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const float fk = __shfl_sync(0xffffffffu, f, s - s0 + k);
+        if (s + k < end)
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] += fk * v[k][e];
+      }
+    }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-#pragma unroll
-  for (int i = 0; i < ROUNDS; ++i) {
-    if (32 * i >= parts) break;
-    const float f = ref[i] == -INFINITY ? 0.0f : EXP2 ? exp2f(ref[i] - m) : expf(ref[i] - m);
-    l += f * sum[i];
-    if (d < 32 && lane + 32 * i < SH_MAX_PARTS) f_s[lane + 32 * i] = f;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  __syncthreads();
-  float acc = 0.0f;
-#pragma unroll
-  for (int s = 0; s < AHEAD; ++s)
-    if (s < parts) acc += f_s[s] * v[s];
-#pragma unroll 8
-  for (int s = AHEAD; s < parts; ++s) acc += f_s[s] * src[s * (HD + 2) + d];
-  const float result = acc / l;
-  store(result);
+  store(l);
   if constexpr (AGAIN) {
-    if (!__syncthreads_or(!isfinite(result))) return;
-    __shared__ float p_s[PAGE];
-    __shared__ float q_s[HD];
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) bad |= !isfinite(acc[e] / l);
+    if (!__any_sync(0xffffffffu, bad)) return;
     const int* table = a.page_table + (size_t)a.seq_slot[row] * a.table_stride;
     const float scale = EXP2 ? a.scale * 0.6931471805599453f : a.scale;
-    q_s[d] = to_f32(a.q[head * HD + d]);
-    float m = -INFINITY, l = 0.0f, acc = 0.0f;
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+#pragma unroll 1
     for (int col = span.first; col < span.first + span.common + span.own; ++col) {
       const size_t slab = (size_t)table[col] * a.nkv + kvh;
       const int from = max(span.lo - col * PAGE, 0), to = min(span.len - col * PAGE, PAGE);
-      __syncthreads();
-      for (int k = from + d; k < to; k += HD) {
+      float sc[2], top = m;        // the scores of keys `lane` and `lane` + 32
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int k = lane + 32 * i;
+        sc[i] = -INFINITY;
+        if (k < from || k >= to) continue;
         const T* key = k_pages + (slab * PAGE + k) * HD;
-        float s = 0.0f;
-        for (int e = 0; e < HD; ++e) s = fmaf(q_s[e], to_f32(key[e]), s);
-        p_s[k] = s * scale;
+        float x = 0.0f;
+#pragma unroll 1
+        for (int d = 0; d < HD; ++d) x = fmaf(to_f32(a.q[head * HD + d]), to_f32(key[d]), x);
+        sc[i] = x * scale;
+        top = fmaxf(top, sc[i]);
       }
-      __syncthreads();
-      float top = m;
-      for (int k = from; k < to; ++k) top = fmaxf(top, p_s[k]);
-      const float alpha = m == top ? 1.0f : expf(m - top);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float old = m == top ? 1.0f : expf(m - top);
       m = top;
-      l *= alpha;
-      acc *= alpha;
-      const T* value = v_pages + (slab * HD + d) * PAGE;
+      l *= old;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= old;
+      const T* value = v_pages + (slab * HD + d0) * PAGE;
+#pragma unroll 1
       for (int k = from; k < to; ++k) {
-        const float w = expf(p_s[k] - m);
+        const float w = expf(__shfl_sync(0xffffffffu, k < 32 ? sc[0] : sc[1], k & 31) - m);
         l += w;
-        acc = fmaf(w, to_f32(value[k]), acc);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(w, to_f32(value[e * PAGE + k]), acc[e]);
       }
     }
-    store(acc / l);
+    store(l);
   }
 }
 
@@ -279,35 +304,20 @@ typedef CUresult (*ShEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, vo
                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// rows x cols numbers of `size` bytes (2: bfloat16, 4: 32-bit), contiguous rows; boxes of 128 bytes x box_rows, 128-byte swizzle.  What is
-// kept by address is the map, which is a function of the address and the sizes alone.
+// rows x cols numbers of `size` bytes (2: bfloat16, 4: 32-bit), contiguous rows; boxes of 128 bytes x box_rows, 128-byte swizzle.
 static bool sh_make_map(CUtensorMap* map, const void* ptr, long long rows, long long cols, int box_rows, int size) {
-  typedef std::tuple<const void*, long long, long long, int, int> Key;
-  static std::map<Key, CUtensorMap> cache;
-  static std::mutex mu;
-  static ShEncodeFn fn = nullptr;
-  std::lock_guard<std::mutex> lock(mu);
-  const Key key(ptr, rows, cols, box_rows, size);
-  auto it = cache.find(key);
-  if (it != cache.end()) { *map = it->second; return true; }
-  if (!fn) {
+  static const ShEncodeFn fn = [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
-      return false;
-    fn = (ShEncodeFn)p;
-  }
+      p = nullptr;
+    return (ShEncodeFn)p;
+  }();
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)cols * size};
   cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
-  CUtensorMap m;
-  if (fn(&m, size == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(ptr), dims, strides, box,
-         estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-    return false;
-  if (cache.size() > 4096) cache.clear();
-  cache[key] = m;
-  *map = m;
-  return true;
+  return fn && fn(map, size == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(ptr), dims, strides,
+                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }

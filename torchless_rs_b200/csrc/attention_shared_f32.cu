@@ -348,7 +348,7 @@ static int sf_run(const void* k_pages, const void* v_pages, long long n_pages, c
                  : R <= 16 ? sf_launch<HD, 2>(tk, tv, a, blocks, stream)
                            : sf_launch<HD, 4>(tk, tv, a, blocks, stream);
   if (st) return st;
-  return tl_launch(attn_shared_merge_kernel<HD, false, false, float>, dim3(a.nh, group_rows, a.groups), dim3(HD), 0, stream, a,
+  return tl_launch(attn_shared_merge_kernel<HD, false, false, float>, dim3((a.nh * (HD / 64) + 3) / 4, group_rows, a.groups), dim3(SH_MERGE_THREADS), 0, stream, a,
                    (const float*)nullptr, (const float*)nullptr);
 }
 
