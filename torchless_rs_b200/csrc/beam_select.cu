@@ -103,10 +103,6 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, int V, const fl
   const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t slot = (size_t)row * gridDim.x + blockIdx.x;
   const float score = scores[row];
-  if (!(score > -INFINITY)) {     // no beam: its row is not read
-    if (tid == 0) part[slot] = {0.0, -INFINITY, 0};
-    return;
-  }
   // The entries in fours on 16-byte boundaries of memory: `shift` entries before the row's first belong to the row before.
   const float* x0 = logits + (size_t)row * ld;
   const int shift = (int)(((uintptr_t)x0 >> 2) & 3);
@@ -140,6 +136,10 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, int V, const fl
 
   float x[16];
   load(first, x);
+  if (!(score > -INFINITY)) {     // no beam: its row does not matter (but its first tile is on its way while the score is)
+    if (tid == 0) part[slot] = {0.0, -INFINITY, 0};
+    return;
+  }
   {
     float best = -INFINITY;
     int best_j = 0;
@@ -326,18 +326,40 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, int V, const fl
   }
 }
 
-struct BsCand {
-  double v;
+// A candidate's value as a word that orders as it does; 0: none.  Both zeros are one.
+struct __align__(16) BsCand {
+  u64 v;
   uint32_t at;          // beam * V + token
 };
-__device__ __forceinline__ bool bs_before(const BsCand& a, const BsCand& b) { return a.v > b.v || (a.v == b.v && a.at < b.at); }
+__device__ __forceinline__ u64 bs_key64(double x) {
+  const u64 u = (u64)__double_as_longlong(x + 0.0);
+  return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double bs_value64(u64 k) { return __longlong_as_double((long long)(k >> 63 ? k & 0x7fffffffffffffffull : ~k)); }
+__device__ __forceinline__ bool bs_before(const BsCand& a, const BsCand& b) { return (a.v > b.v) | ((a.v == b.v) & (a.at < b.at)); }
+// How many of list[0 .. c) come before `mine`.  (Eight loads, then comparisons without branches: taken one by one, with the second half of a
+// comparison only where the first ties, 32 of them took 7000 cycles and the whole selection half as long again.)
+__device__ __forceinline__ int bs_rank(const BsCand* list, int c, const BsCand& mine) {
+  int rank = 0, k = 0;
+  for (; k + 8 <= c; k += 8) {
+    BsCand o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = list[k + i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rank += bs_before(o[i], mine) ? 1 : 0;
+  }
+#pragma unroll 1
+  for (; k < c; ++k) rank += bs_before(list[k], mine) ? 1 : 0;
+  return rank;
+}
 __device__ __forceinline__ BsCand bs_shfl(const BsCand& a, int o) {
   return {__shfl_xor_sync(0xffffffffu, a.v, o), __shfl_xor_sync(0xffffffffu, a.at, o)};
 }
 
-// CAND: candidates of a sequence per thread that are held in registers; 0: any number, read again for every look at them.
+// CAND: candidates of a sequence per thread that are held in registers; 0: any number, read again for every look at them.  (The bound on
+// registers is for the order of the code: without it 64 sequences of 8 beams take 4 us more.)
 template <int GS, int CAND>
-__global__ void __launch_bounds__(BS_THREADS)
+__global__ void __launch_bounds__(BS_THREADS, 4)
 beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ cand, const float* __restrict__ scores, int B, int V,
                   int n, int parts, float* __restrict__ values, int* __restrict__ beams, int* __restrict__ tokens) {
   constexpr int GROUPS = BS_THREADS / GS, HELD = CAND ? CAND : 1;
@@ -350,26 +372,31 @@ beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ can
   const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t row0 = (size_t)s * B;
   const int total = B * parts * n;
-  const BsCand none = {-INFINITY, 0xffffffffu};
+  const BsCand none = {0, 0xffffffffu};
   if (tid == 0) count = 0;
   pdl_wait();
   pdl_launch_dependents();
   // candidate i: its value without its beam's share, and which beam's; everything is on its way before the first is waited for
   struct Raw {
     float x, score;
-    int beam;                             // -1: none
+    int beam, left;                       // left: how many follow it and itself; none if it is not positive
     uint32_t token;
   };
   auto raw = [&](int i) -> Raw {
-    if (i >= total) return {0.0f, 0.0f, -1, 0u};
+    if (i >= total) return {0.0f, 0.0f, 0, 0, 0u};
     const int k = i / n, b = k / parts;
     const uint2 c = cand[row0 * parts * n + i];
-    return {bs_value(c.x), scores[row0 + b], i - k * n < part[row0 * parts + k].count ? b : -1, c.y};
+    return {bs_value(c.x), scores[row0 + b], b, part[row0 * parts + k].count - (i - k * n), c.y};
   };
   auto value = [&](const Raw& r) -> BsCand {
-    if (r.beam < 0) return none;
-    return {(double)r.score + ((double)r.x - lse[r.beam]), (uint32_t)r.beam * (uint32_t)V + r.token};
+    if (r.left <= 0) return none;
+    return {bs_key64((double)r.score + ((double)r.x - lse[r.beam])), (uint32_t)r.beam * (uint32_t)V + r.token};
   };
+  auto part_of = [&](int b) -> BsPart {
+    if (b < B && lane < parts) return part[(row0 + b) * parts + lane];
+    return {0.0, -INFINITY, 0};
+  };
+  BsPart q = part_of(warp);
   Raw held[HELD];
   if (CAND) {
 #pragma unroll
@@ -378,8 +405,6 @@ beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ can
   // a warp per row: its maximum, its sum
   for (int b = warp; b < B; b += BS_THREADS / 32) {
     const BsPart* p = part + (row0 + b) * parts;
-    BsPart q = {0.0, -INFINITY, 0};
-    if (lane < parts) q = p[lane];
     float M = q.max;
     for (int i = lane + 32; i < parts; i += 32) M = fmaxf(M, p[i].max);
 #pragma unroll
@@ -394,6 +419,7 @@ beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ can
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
     if (lane == 0) lse[b] = (double)M + log(sum);       // (a row without entries: not used)
+    q = part_of(b + BS_THREADS / 32);
   }
   __syncthreads();
   BsCand mine[HELD], best = none;
@@ -414,13 +440,12 @@ beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ can
     const BsCand other = bs_shfl(best, o);
     if (bs_before(other, best)) best = other;
   }
+  if (best.v == 0) best.at = 0xffffffffu - tid / GS;       // (empty groups come one after the other)
   if (tid % GS == 0) gm[tid / GS] = best;
   __syncthreads();
   if (tid < GROUPS) {
     const BsCand of = gm[tid];
-    int rank = 0;
-#pragma unroll 4
-    for (int k = 0; k < GROUPS; ++k) rank += bs_before(gm[k], of) || (k < tid && gm[k].at == of.at) ? 1 : 0;   // (empty groups are equal)
+    const int rank = bs_rank(gm, GROUPS, of);
     if (rank == (n < GROUPS ? n : GROUPS) - 1) bound = of;
   }
   __syncthreads();
@@ -441,9 +466,10 @@ beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ can
   const int c = count;
   const size_t o0 = (size_t)s * n;
   auto put = [&](int r, const BsCand& e) {
-    const bool got = e.at != 0xffffffffu && e.v > -INFINITY;
+    const double v = bs_value64(e.v);
+    const bool got = e.at != 0xffffffffu && v > -INFINITY;
     const uint32_t beam = e.at / (uint32_t)V;
-    values[o0 + r] = got ? (float)e.v : -INFINITY;
+    values[o0 + r] = got ? (float)v : -INFINITY;
     beams[o0 + r] = got ? (int)beam : -1;
     tokens[o0 + r] = got ? (int)(e.at - beam * (uint32_t)V) : -1;
   };
@@ -453,14 +479,13 @@ beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ can
       int rank = i;                       // places without a candidate
       if (i < c) {
         e = buf[i];
-        rank = 0;
-        for (int k = 0; k < c; ++k) rank += bs_before(buf[k], e) ? 1 : 0;
+        rank = bs_rank(buf, c, e);
       }
       if (rank < n) put(rank, e);
     }
   } else {
     // more reach the bound than there is room for (they bunch in few threads): one after the other
-    BsCand last = {INFINITY, 0u};
+    BsCand last = {~0ull, 0u};
     for (int r = 0; r < n; ++r) {
       BsCand m = none;
       for (int i = tid; i < total; i += BS_THREADS) {

@@ -24,7 +24,7 @@ class BeamSelector:
 
         `logits` [sequences * beams, vocabulary]: the step's logits, a sequence's beams in consecutive rows;
         `scores` [sequences, beams]: each beam's log-probability so far, -inf for a place without a beam (its row of
-        logits is not read).  Returns (values, beams, tokens), each [sequences, n] on the device, in falling order of
+        logits does not matter).  Returns (values, beams, tokens), each [sequences, n] on the device, in falling order of
         scores[s, b] + log softmax(logits[s, b])[t]; of equal ones the lower beam, then the lower token, comes first.
         The order is decided in 64 bits, the values are rounded to 32.  A logit that is NaN or -inf is no continuation, +inf
         counts as the largest finite number; where fewer than `n` continuations exist, the last places hold -inf, -1, -1.
