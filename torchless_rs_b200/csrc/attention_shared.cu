@@ -26,12 +26,13 @@
 // memory and returns.
 #include <cuda.h>
 #include <stdlib.h>
+#include <type_traits>
 
 #include "attention_bf16_common.cuh"
 #include "attention_shared.cuh"
 
 #define SH_SOFT 256                                 // threads of the softmax: warps 0-3 the lower half of the columns, 4-7 the upper
-#define SH_THREADS (SH_SOFT + 64)                   // warp 8 TMA, warp 9 tcgen05.mma
+#define SH_THREADS (SH_SOFT + 96)                   // warp 8 TMA of keys, warp 9 of values, warp 10 tcgen05.mma
 #define SH_KSUB (HEAD_DIM / 64)                     // 64-column boxes of a K slab
 #define SH_PAGE_K (PAGE * HEAD_DIM * 2)
 #define SH_PAGE_V (HEAD_DIM * PAGE * 2)
@@ -92,13 +93,19 @@ __device__ __forceinline__ uint32_t sh_mask(int c0, int c1) {
 }
 // s <- s scale - reference in the columns that see this thread's key, -inf in the others; returns the largest.
 template <bool MASKED, int N>
-__device__ __forceinline__ float sh_shift(float (&s)[N], uint32_t columns, const float (&neg_ref)[N], float scale) {
+__device__ __forceinline__ float sh_shift(float (&s)[N], uint32_t columns, const float* neg_ref, float scale) {
   float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-  for (int c = 0; c < N; ++c) {
-    s[c] = fmaf(s[c], scale, neg_ref[c]);
-    if (MASKED) s[c] = (columns >> c & 1u) ? s[c] : -INFINITY;
-    if (c & 1) m1 = fmaxf(m1, s[c]); else m0 = fmaxf(m0, s[c]);
+  for (int c4 = 0; c4 < N; c4 += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(neg_ref + c4);
+    const float neg[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = c4 + e;
+      s[c] = fmaf(s[c], scale, neg[e]);
+      if (MASKED) s[c] = (columns >> c & 1u) ? s[c] : -INFINITY;
+      if (c & 1) m1 = fmaxf(m1, s[c]); else m0 = fmaxf(m0, s[c]);
+    }
   }
   return fmaxf(m0, m1);
 }
@@ -175,6 +182,7 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   // [2][3]: a reference in this half of the columns has to move.  By tile number modulo 3: written before a tile's barrier, read after
   // it, cleared behind the next one (what a warp that runs ahead writes by then is another tile's).
   volatile int* moved_s = abort_flag + 1;
+  ShPiece* first_s = (ShPiece*)(abort_flag + 1 + 6);   // the stretch's first unit
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (smem_u32(sh_smem) & 1023u) {                     // nothing has been allocated yet
@@ -195,61 +203,105 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (tid == 32) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_v) : "memory");
+  }
   if (warp == 0) {
     tmem_alloc(tmem_slot, Z::tmem);
     tmem_relinquish();
   }
   pdl_wait();
   pdl_launch_dependents();
-  if (warp == 8) sh_make_line<2>(table, total_s, a, gridDim.x, lane);
+  // The next piece with tiles from place t on; without, if there is none.  (The first one is found once for all roles: this is much code,
+  // and every copy of it that runs is fetched from afar.)
+  int gap = 0, share = 0, t0 = 0, t1 = 0;
+  auto piece = [&](int t) {
+    ShPiece p = {};
+    while (t < t1) {
+      p = sh_locate(table, a, gap, t, t1);
+      t = p.next;
+      if (p.tile < p.last) break;
+    }
+    return p;
+  };
+  auto stretch = [&] {
+    gap = total_s[2];
+    share = sh_share(total_s, gridDim.x, a.parts);
+    t0 = min((int)blockIdx.x * share, total_s[0]);
+    t1 = min(t0 + share, total_s[0]);
+  };
+  if (warp == 8) {
+    sh_make_line<2>(table, total_s, a, gridDim.x, lane);
+    __syncwarp();
+    stretch();
+    const ShPiece p = piece(t0);
+    if (lane == 0) *first_s = p;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot, tmem_o = tmem + 2 * N;
-  const int total = total_s[0], gap = total_s[2], share = sh_share(total_s, gridDim.x, a.parts);
-  const int t0 = min((int)blockIdx.x * share, total), t1 = min(t0 + share, total);
+  stretch();
   const int G = a.nh / a.nkv;
 
-  if (t0 < t1) {
-    if (warp == 8 && elect_one()) {
-      // ---- TMA: keys, then values, of every tile of the stretch
-      bool ok = true;
-      int n = 0;
-      for (int t = t0; t < t1 && ok;) {
-        const ShPiece p = sh_locate(table, a, gap, t, t1);
-        t = p.next;
-        for (int j = p.tile; j < p.last && ok; ++j, ++n) {
-          const int pages = min(2, p.pages - 2 * j);
-          int slab[2];
+  // ---- TMA: a warp for the keys of every tile of the stretch, one for the values.  The lanes look up 32 pages at a time:
+  // with one lookup (two reads, each waiting for the one before) before every tile, and values that wait for their slot in front of the next
+  // keys, 4 prompts x 8 beams of the 22B sizes took 4 us more.
+  auto produce = [&](auto which) {
+    constexpr bool VALUES = decltype(which)::value;
+    constexpr int SLOTS = VALUES ? Z::VS : Z::KS, BYTES = VALUES ? SH_PAGE_V : SH_PAGE_K;
+    uint64_t *full = VALUES ? v_full : k_full, *empty = VALUES ? v_empty : k_empty;
+    bool ok = true;
+    int n = 0;
+    ShPiece p = *first_s;
+    for (int i0 = 2 * p.tile; p.tile < p.last && ok;) {
+      const int end = min(min(2 * p.last, p.pages), i0 + 32);
+      int slab = 0;
+      if (i0 + lane < end) {
+        int owner, col;
+        sh_page(p, i0 + lane, owner, col);
+        slab = a.page_table[(size_t)a.seq_slot[p.row0 + max(owner, 0)] * a.table_stride + col] * a.nkv + p.kvh;
+      }
+      for (int i = 0; i0 + i < end; i += 2, ++n) {
+        const int s = n % SLOTS, slab0 = __shfl_sync(0xffffffffu, slab, i), slab1 = __shfl_sync(0xffffffffu, slab, i + 1);
+        ok = __all_sync(0xffffffffu, sh_park(&empty[s], ((uint32_t)(n / SLOTS) & 1u) ^ 1u, abort_flag, VALUES ? 2 : 1));
+        if (!ok) break;
+        if (lane == 0) {
+          const int pages = min(2, end - i0 - i);
+          mbar_expect_tx(&full[s], pages * BYTES);
           for (int h = 0; h < pages; ++h) {
-            int owner, col;
-            sh_page(p, 2 * j + h, owner, col);
-            slab[h] = a.page_table[(size_t)a.seq_slot[p.row0 + max(owner, 0)] * a.table_stride + col] * a.nkv + p.kvh;
-          }
-          const int ks = n % Z::KS, vs = n % Z::VS;
-          ok = sh_park(&k_empty[ks], ((uint32_t)(n / Z::KS) & 1u) ^ 1u, abort_flag, 1);
-          if (!ok) break;
-          mbar_expect_tx(&k_full[ks], pages * SH_PAGE_K);
-          for (int h = 0; h < pages; ++h)
+            const int at = h ? slab1 : slab0;
+            if constexpr (VALUES) {
+              tma_load_2d(v_s + s * Z::V + h * SH_PAGE_V, &tm_v, &full[s], 0, at * HEAD_DIM);
+            } else {
 #pragma unroll
-            for (int sub = 0; sub < SH_KSUB; ++sub)
-              tma_load_2d(k_s + ks * Z::K + sub * (2 * PAGE * 128) + h * (PAGE * 128), &tm_k, &k_full[ks], sub * 64, slab[h] * PAGE);
-          ok = sh_park(&v_empty[vs], ((uint32_t)(n / Z::VS) & 1u) ^ 1u, abort_flag, 2);
-          if (!ok) break;
-          mbar_expect_tx(&v_full[vs], pages * SH_PAGE_V);
-          for (int h = 0; h < pages; ++h) tma_load_2d(v_s + vs * Z::V + h * SH_PAGE_V, &tm_v, &v_full[vs], 0, slab[h] * HEAD_DIM);
+              for (int sub = 0; sub < SH_KSUB; ++sub)
+                tma_load_2d(k_s + s * Z::K + sub * (2 * PAGE * 128) + h * (PAGE * 128), &tm_k, &full[s], sub * 64, at * PAGE);
+            }
+          }
         }
+        __syncwarp();
       }
-      if (!ok) {
-        // given up: what is in flight lands before the block ends, or for as long as a wait may take
-        for (int i = 0; i < Z::KS && i < n; ++i)
-          for (uint32_t k = 0; k < TL_WAIT_LIMIT / 64 && !tl_mbar_try_wait(&k_full[(n - 1 - i) % Z::KS], (uint32_t)((n - 1 - i) / Z::KS) & 1u); ++k) {}
-        for (int i = 0; i < Z::VS && i < n; ++i)
-          for (uint32_t k = 0; k < TL_WAIT_LIMIT / 64 && !tl_mbar_try_wait(&v_full[(n - 1 - i) % Z::VS], (uint32_t)((n - 1 - i) / Z::VS) & 1u); ++k) {}
-        const int ks = n % Z::KS;    // the tile that was given up half way
-        for (uint32_t k = 0; k < TL_WAIT_LIMIT / 64 && !tl_mbar_try_wait(&k_full[ks], (uint32_t)(n / Z::KS) & 1u); ++k) {}
+      i0 += 32;
+      if (i0 >= 2 * p.last) {
+        p = piece(p.next);
+        i0 = 2 * p.tile;
       }
-    } else if (warp == 9 && elect_one()) {
+    }
+    if (!ok && lane == 0) {
+      // given up: what is in flight lands before the block ends, or for as long as a wait may take
+      for (int i = 0; i < SLOTS && i < n; ++i)
+        for (uint32_t k = 0; k < TL_WAIT_LIMIT / 64 && !tl_mbar_try_wait(&full[(n - 1 - i) % SLOTS], (uint32_t)((n - 1 - i) / SLOTS) & 1u); ++k) {}
+    }
+  };
+
+  if (t0 < t1) {
+    if (warp == 8) {
+      produce(std::false_type());
+    } else if (warp == 9) {
+      produce(std::true_type());
+    } else if (warp == 10 && elect_one()) {
       // ---- the products: S^T of tile n + 1 before O^T of tile n
       constexpr uint32_t idesc = sh_idesc(N);
       const uint32_t desc_hi = (uint32_t)(smem_desc_k128(0) >> 32);
@@ -257,25 +309,20 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       auto desc = [&](uint32_t lo) { return ((uint64_t)desc_hi << 32) | lo; };
       const uint32_t k_lo = lo_of(k_s), v_lo = lo_of(v_s), q_lo = lo_of(q_s), p_lo = lo_of(p_s);
       // tile n + 1's unit runs ahead of tile n's
-      int s_unit = 0, s_left = 0, s_t = t0;       // for S^T: units begun, tiles left of the current one, the next piece's place
-      int o_unit = 0, o_left = 0, o_t = t0, o_tile = 0;
-      ShPiece o_piece = {};
-      bool o_first = false;
-      auto piece = [&](int& t) {                  // the next piece with tiles; without, if there is none
-        ShPiece p = {};
-        while (t < t1) {
-          p = sh_locate(table, a, gap, t, t1);
-          t = p.next;
-          if (p.tile < p.last) break;
-        }
-        return p;
-      };
+      ShPiece s_piece = *first_s, o_piece = s_piece;
+      int s_unit = 0, s_left = s_piece.last - s_piece.tile;            // for S^T: units begun, tiles left of the current one
+      int o_unit = 0, o_tile = o_piece.tile;
+      bool s_begins = true, o_first = true;
       // 1: issued, 0: there is no further tile, -1: given up
       auto scores = [&](int n) {
         if (s_left == 0) {
-          const ShPiece p = piece(s_t);
-          s_left = p.last - p.tile;
+          s_piece = piece(s_piece.next);
+          s_left = s_piece.last - s_piece.tile;
           if (s_left == 0) return 0;
+          s_begins = true;
+        }
+        if (s_begins) {
+          s_begins = false;
           if (!sh_park(&q_full[s_unit & 1], (uint32_t)(s_unit >> 1) & 1u, abort_flag, 3)) return -1;
           ++s_unit;
         }
@@ -291,15 +338,11 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         umma_commit(&k_empty[n % Z::KS]);
         return 1;
       };
-      int ready = scores(0);                      // whether tile n's scores have been issued
-      for (int n = 0; ready == 1; ++n) {
-        ready = scores(n + 1);                    // (its buffer was read before P of tile n - 1 was there)
-        if (ready < 0) break;
-        if (o_left == 0) {
-          o_piece = piece(o_t);
-          o_left = o_piece.last - o_piece.tile;
-          o_tile = o_piece.tile;
-          o_first = true;
+      for (int n = -1; s_piece.tile < s_piece.last || n >= 0; ++n) {
+        const int next = scores(n + 1);           // (its buffer was read before P of tile n - 1 was there)
+        if (next < 0) break;
+        if (n < 0) continue;
+        if (o_first) {
           // O^T is free when the unit before has been written out
           if (o_unit > 0 && !sh_park(o_free, (uint32_t)(o_unit - 1) & 1u, abort_flag, 5)) break;
           ++o_unit;
@@ -318,8 +361,12 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           }
         umma_commit(&pv_done[n & 1]);
         umma_commit(&v_empty[n % Z::VS]);
-        --o_left;
-        ++o_tile;
+        if (next == 0) break;
+        if (++o_tile == o_piece.last) {
+          o_piece = piece(o_piece.next);
+          o_tile = o_piece.tile;
+          o_first = true;
+        }
       }
     } else if (warp < 8) {
       // ---- softmax: key `key` of a tile, columns first_col to first_col + NC - 1.  A wait that runs out leaves the loop's barriers in
@@ -347,31 +394,15 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         sh_arrive(&q_full[buf]);
       };
       int n = 0, unit = 0;
-      float l[NC], neg_ref[NC];                // sums of this thread's weights; the negated references (0: none yet)
-      auto load_refs = [&] {
-#pragma unroll
-        for (int c = 0; c < NC; c += 4) {
-          const float4 r = *reinterpret_cast<const float4*>(neg_s + first_col + c);
-          neg_ref[c] = r.x; neg_ref[c + 1] = r.y; neg_ref[c + 2] = r.z; neg_ref[c + 3] = r.w;
-        }
-      };
-      int t = t0;
-      auto piece = [&] {                       // the next piece with tiles; without, if there is none
-        ShPiece p = {};
-        while (t < t1) {
-          p = sh_locate(table, a, gap, t, t1);
-          t = p.next;
-          if (p.tile < p.last) break;
-        }
-        return p;
-      };
-      ShPiece p = piece();
+      float l[NC];                             // sums of this thread's weights
+      const float* neg = neg_s + first_col;    // (the negated references stay in shared memory: 32 columns of them are registers too many)
+      ShPiece p = *first_s;
       if (p.tile < p.last) load_q(p, 0);
       for (; p.tile < p.last; ++unit) {
         const int last = p.last, R = p.beams * G;
         ShPiece np = {};
 #pragma unroll
-        for (int c = 0; c < NC; ++c) l[c] = neg_ref[c] = 0.0f;
+        for (int c = 0; c < NC; ++c) l[c] = 0.0f;
         if (key < NC) {
           ref_s[first_col + key] = -INFINITY;
           neg_s[first_col + key] = 0.0f;
@@ -379,17 +410,35 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         sh_bar(upper);
         const uint32_t all = sh_mask(0, min(max(R - first_col, 0), NC));
         uint32_t is_set = 0;                   // columns that have a reference
-        // this thread's page of the tile, step by step
-        int owner = -1, in_own = 0, col = p.first + 2 * p.tile + page_of;
-        if (2 * p.tile + page_of >= p.common) {
-          owner = p.own ? (2 * p.tile + page_of - p.common) / p.own : 0;
-          in_own = 2 * p.tile + page_of - p.common - owner * p.own;
-          col = p.first + p.common + in_own;
+        // the tile's two pages, step by step
+        struct { int owner, in_own, col; } page[2];
+        page[0] = {-1, 0, p.first + 2 * p.tile};
+        if (2 * p.tile >= p.common) {
+          page[0].owner = p.own ? (2 * p.tile - p.common) / p.own : 0;
+          page[0].in_own = 2 * p.tile - p.common - page[0].owner * p.own;
+          page[0].col = p.first + p.common + page[0].in_own;
         }
+        auto step = [&](int to, int from) {
+          int owner = page[from].owner, in_own = page[from].in_own, col = page[from].col + 1;
+          if (owner < 0) {
+            if (col == p.first + p.common) owner = 0;
+          } else if (++in_own >= p.own) {
+            in_own = 0;
+            ++owner;
+            col = p.first + p.common;
+          }
+          page[to] = {owner, in_own, col};
+        };
+        step(1, 0);
+        // the columns that see a page, of this half
+        auto seen_by = [&](int owner) {
+          return owner < 0 ? all : sh_mask(min(max(owner * G - first_col, 0), NC), min(max(owner * G + G - first_col, 0), NC));
+        };
         for (int j = p.tile; j < last; ++j, ++n) {
           const int buf = n & 1, now3 = n % 3;
           const bool there = 2 * j + page_of < p.pages;
-          const uint32_t columns = owner < 0 ? all : sh_mask(min(max(owner * G - first_col, 0), NC), min(max(owner * G + G - first_col, 0), NC));
+          const int owner = page_of ? page[1].owner : page[0].owner, col = page_of ? page[1].col : page[0].col;
+          const uint32_t columns = seen_by(owner);
           const int at = col * PAGE + (key & 63);
           const bool seen = there && at >= p.lo && at < p.len;
           const bool plain = there && owner < 0 && col * PAGE >= p.lo && col * PAGE + PAGE <= p.len;
@@ -404,10 +453,8 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               if (2 * j + h >= p.pages) continue;
-              int ow, cl;
-              sh_page(p, 2 * j + h, ow, cl);
-              of[h] = (ow < 0 ? all : sh_mask(min(max(ow * G - first_col, 0), NC), min(max(ow * G + G - first_col, 0), NC))) & ~is_set;
-              if (of[h] && key == h * PAGE + max(p.lo - cl * PAGE, 0)) {
+              of[h] = seen_by(page[h].owner) & ~is_set;
+              if (of[h] && key == h * PAGE + max(p.lo - page[h].col * PAGE, 0)) {
 #pragma unroll
                 for (int c = 0; c < NC; c += 4)
                   *reinterpret_cast<float4*>(new_s + h * N + first_col + c) = make_float4(s[c], s[c + 1], s[c + 2], s[c + 3]);
@@ -423,11 +470,10 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
                 neg_s[first_col + key] = -ref;
               }
               sh_bar(upper);
-              load_refs();
               is_set |= of[0] | of[1];
             }
           }
-          const float largest = plain ? sh_shift<false>(s, columns, neg_ref, a.scale) : sh_shift<true>(s, seen ? columns : 0u, neg_ref, a.scale);
+          const float largest = plain ? sh_shift<false>(s, columns, neg, a.scale) : sh_shift<true>(s, seen ? columns : 0u, neg, a.scale);
           if (__any_sync(0xffffffffu, largest > SH_SLACK) && lane == 0) moved[now3] = 1;
           sh_bar(upper);
           if (key == 0) moved[(n + 2) % 3] = 0;
@@ -447,11 +493,10 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
               al_s[first_col + key] = now == old ? 1.0f : sh_ex2(old - now);
             }
             sh_bar(upper);
-            load_refs();
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
               l[c] *= al_s[first_col + c];
-              s[c] += neg_ref[c];
+              s[c] += neg[c];
             }
             if (j > p.tile) {
               // O^T so far, once the product before is done (the next one waits for this tile's weights)
@@ -481,21 +526,11 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           sh_arrive(&p_full[buf]);
           if (j == p.tile) {
             // the next unit's queries: its buffer's scores were all read a unit ago
-            np = piece();
+            np = piece(p.next);
             if (np.tile < np.last) load_q(np, (unit + 1) & 1);
           }
-          // two pages on
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            ++col;
-            if (owner < 0) {
-              if (col == p.first + p.common) { owner = 0; in_own = 0; }
-            } else if (++in_own >= p.own) {
-              in_own = 0;
-              ++owner;
-              col = p.first + p.common;
-            }
-          }
+          step(0, 1);
+          step(1, 0);
         }
         // ---- the unit's end: sums over the keys, O^T out
         sh_columns<NC>(l, lane, red_s + quad * N + first_col, [](float x, float y) { return x + y; });
