@@ -10,16 +10,23 @@
 // tensor cores keys take the 128 lanes and rows the columns, so that few rows cost little:
 //   S^T[128 keys, N]  = K . Q^T      two pages of keys, Q in shared memory, S^T in tensor memory (two buffers)
 //   softmax           a key and half of the columns per thread; a column's reference is the score of the first key that it sees and
-//                     moves only when another exceeds it by 2^60, so that a tile needs one barrier of four warps and no maxima; P^T rounded to bfloat16 (2^-9 of each weight) to shared memory
+//                     moves only when another exceeds it by 2^60, so that a tile needs one barrier of four warps and no maxima; P^T
+//                     rounded to bfloat16 (by at most 2^-8 of each weight: the products take bfloat16) to shared memory
 //   O^T[hd, N]       += V^T . P^T    the transposed value slab as it lies in the cache, O^T in tensor memory
 // A row's own page is multiplied with all rows of the unit; the others' weights are zero there, as all weights of keys that are not seen
 // are.  Where such a value is no number (0 x NaN is NaN) the second kernel finds a result that is none and computes it again,
 // from the keys that the row sees alone.
 //
 // The tiles of all units lie in one line, which the blocks (one per SM) cut into equal stretches: nobody waits for the longest
-// sequence, and loads run on across units.  A stretch of a unit leaves a reference, a sum and a
-// weighted sum per row and head, and a second kernel merges them in the order of the keys.  What bounds this is the memory: a tile of head
-// size 128 is 64 KB and takes an SM 1.5 us at the copy rate; its softmax and products take about a third of that.
+// sequence, and loads run on across units.  A stretch of a unit leaves a reference, a sum and a weighted sum per row and head, and a
+// second kernel merges them in the order of the keys.
+//
+// What bounds this is the memory: a tile of head size 128 is 64 KB and takes an SM 1.5 us at the copy rate; the softmax of 16 columns
+// takes a third of that, of 64 columns 1.1 us.  Measured (L2 cold): 4 prompts of 6000 to 16000 tokens x 8 beams, 48 over 8 heads of 128, 206 MB:
+// 47 us, 1.55 us a tile between a start of 5 us (the line, the lists of pages, the first pages) and an end of 5 (a unit's results 2, the
+// merge 3); 8 prompts of 300 to 4000 tokens x 4, 32 over 8 heads, 84 MB: 24 us; one prompt of 2000 x 4: 10 us, all of it start and
+// end; heads of 64, 6 prompts x 16 beams: 18 us, its tiles 32 KB with a softmax of 64 columns.  Sixteen warps of softmax for 64 columns
+// instead of eight: 2 us more (registers).
 //
 // Nothing is read before the wait for the kernels before: a page may have been copied by one of them.  Every wait on an mbarrier
 // is bounded; when a bound is hit the block records a code in tl_attn_shared_error, waits (bounded) for its copies in flight, frees its tensor
@@ -382,13 +389,20 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         uint8_t* dst = q_s + buf * Z::Q;
         constexpr int C = HEAD_DIM / 8;        // 16-byte pieces of a row
         const int c = tid % C;
+        constexpr int STEP = SH_SOFT / C, PASSES = (N + STEP - 1) / STEP;
         ShRow at = q_row;
-#pragma unroll 1
-        for (int r = tid / C; r < N; r += SH_SOFT / C) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (r < p.beams * G) v = ldg16(a.q + ((size_t)(p.row0 + at.beam) * a.nh + p.kvh * G + at.head) * HEAD_DIM + c * 8);
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * (N * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
-          at.step(SH_SOFT / C);
+        uint4 v[PASSES];                       // (all on their way before the first is waited for)
+#pragma unroll
+        for (int k = 0; k < PASSES; ++k) {
+          v[k] = make_uint4(0, 0, 0, 0);
+          if (tid / C + k * STEP < p.beams * G)
+            v[k] = ldg16(a.q + ((size_t)(p.row0 + at.beam) * a.nh + p.kvh * G + at.head) * HEAD_DIM + c * 8);
+          at.step(STEP);
+        }
+#pragma unroll
+        for (int k = 0; k < PASSES; ++k) {
+          const int r = tid / C + k * STEP;
+          if (r < N) *reinterpret_cast<uint4*>(dst + (c >> 3) * (N * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
         }
         sh_async_fence();
         sh_arrive(&q_full[buf]);

@@ -70,9 +70,9 @@ template <int TP>
 __device__ __forceinline__ int sh_tiles(int common, int own, int beams) { return (common + own * beams + TP - 1) / TP; }
 
 // One warp: the groups' places in the line.  Every unit begins with `totals[2]` places without a tile: that is what beginning a unit and
-// writing one out takes a block, in tiles, so that equal stretches take equal time (22B sizes, 4 prompts x 8 beams: blocks with one unit
-// 39 us and with two 50 us without them).  Where a stretch is a few tiles long there are none: more, shorter stretches are then
-// faster.  totals[0], [1]: places in the line, tiles of the longest unit.
+// writing one out takes a block, in tiles, so that equal stretches take equal time (4 prompts x 8 beams of the 22B
+// sizes: 57.8 us without them, 55.8 with 2, 53.6 with 4, 52.5 with 6; 8 x 4 of the 7B sizes 27.4, 26.5, 26.9,
+// 27.2).  Where a stretch is a few tiles long there are fewer: more, shorter stretches are then faster.  totals[0], [1]: places in the line, tiles of the longest unit.
 template <int TP, typename T>
 __device__ __forceinline__ void sh_make_line(ShGroup* table, int* totals, const ShArgs<T>& a, int blocks, int lane) {
   int tiles = 0, units = 0, longest = 0;

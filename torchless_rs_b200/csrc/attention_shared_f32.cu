@@ -9,6 +9,9 @@
 // 1.1 us at the SM's full rate, 32 rows 2.1 us.  Pages come by TMA, keys in boxes of 32 dimensions and values in boxes of 32 keys,
 // whose 128-byte swizzle keeps the reads of neighbouring rows in different banks.  Two blocks share an SM (one's barriers and
 // softmax under the other's products); the next page's keys are requested when the scores are done, its values after the products.
+// Measured: 4 prompts of 500 to 2000 tokens x 4 beams, 32 over 8 heads of 128, 51 MB: 30 us; an SM issues 1.8 instructions a cycle of 4, 59 % of
+// them multiply-adds (eight warps of 128 registers do not hide the reads of shared memory and the four barriers of a page).  One
+// block per SM with two buffers for pages: 35 us.
 //
 // Nothing is read before the wait for the kernels before: a page may have been copied by one of them.  Every wait on an mbarrier
 // is bounded; when a bound is hit the block records a code in tl_attn_shared_f32_error, waits (bounded) for its copies in flight and returns.
@@ -121,14 +124,19 @@ attn_shared_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   const int dg = tid % DG, kv = (tid / DG) % KV, ro = tid / (DG * KV);
   const ShRow row_of(tid / DG, G), soft_row(sr, G), out_row(tid / HD, G);
   auto load_q = [&](const ShPiece& p) {
+    constexpr int STEP = SF_THREADS / DG, PASSES = (ROWS + STEP - 1) / STEP;
     ShRow at = row_of;
-#pragma unroll 1
-    for (int r = tid / DG; r < ROWS; r += SF_THREADS / DG) {
-      reinterpret_cast<float4*>(q_s)[r * DG + dg] =
-          r < p.beams * G ? reinterpret_cast<const float4*>(a.q + ((size_t)(p.row0 + at.beam) * a.nh + p.kvh * G + at.head) * HD)[dg]
-                          : make_float4(0.f, 0.f, 0.f, 0.f);
-      at.step(SF_THREADS / DG);
+    float4 v[PASSES];              // (all on their way before the first is waited for)
+#pragma unroll
+    for (int k = 0; k < PASSES; ++k) {
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (tid / DG + k * STEP < p.beams * G)
+        v[k] = reinterpret_cast<const float4*>(a.q + ((size_t)(p.row0 + at.beam) * a.nh + p.kvh * G + at.head) * HD)[dg];
+      at.step(STEP);
     }
+#pragma unroll
+    for (int k = 0; k < PASSES; ++k)
+      if (tid / DG + k * STEP < ROWS) reinterpret_cast<float4*>(q_s)[(tid / DG + k * STEP) * DG + dg] = v[k];
   };
   // A wait that runs out leaves the loop's barriers in place: the warps go through them to the end (every later wait returns at
   // once), and what they write is not valid.
@@ -183,9 +191,8 @@ attn_shared_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           }
         }
         // the KS shares: every exchange halves how many scores a thread holds; thread ks ends with those from ks * 32 / KS on
-        // (the lanes that exchange have one rs)
+        // (rs is one for a warp)
         int half = 16;
-        const unsigned lanes = __activemask();
 #pragma unroll
         for (int mask = KS / 2; mask > 0; mask >>= 1, half >>= 1) {
           const bool up = (ks & mask) != 0;
@@ -193,7 +200,7 @@ attn_shared_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           for (int j = 0; j < 16; ++j) {
             if (j < half) {
               const float send = up ? sc[j] : sc[j + half], keep = up ? sc[j + half] : sc[j];
-              sc[j] = keep + __shfl_xor_sync(lanes, send, mask);
+              sc[j] = keep + __shfl_xor_sync(0xffffffffu, send, mask);
             }
           }
         }
