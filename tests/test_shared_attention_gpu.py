@@ -239,6 +239,31 @@ def test_a_call_that_does_not_say_that_pages_are_shared_gives_the_same():
     ops.check_kernel_errors()
 
 
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("window", [None, 200])
+@pytest.mark.parametrize("begun", [([3, 130], [0, 2]), ([64, 1024], [1, 16]), ([1, 1], [0, 0])])
+def test_a_recorded_call_is_right_for_lengths_that_came_later(dtype, nh, nkv, hd, window, begun):
+    """Recorded at other lengths and common pages than it is replayed with; `bound` covers what the common pages come to."""
+    s = Setting(dtype, nh, nkv, hd, [4, 3], [450, 1100], [6, 16], window=window, seed=3)
+    lens, pages = s.seq_len.clone(), s.group_pages.clone()
+    out = torch.full_like(s.q, 7.0)
+    of = dict(out=out, lens=begun[0], shared=begun[1], bound=18)
+    row_len = [min(n, m) for b, n, m in zip(s.beams, begun[0], s.lens) for _ in range(b)]
+    s.seq_len.copy_(torch.tensor(row_len, dtype=torch.int32))
+    s.group_pages.copy_(torch.tensor(begun[1], dtype=torch.int32))
+    if window:                                        # (pages before the window are not in the tables)
+        s.group_pages.copy_(pages)
+        s.seq_len.copy_(lens)
+    s.run(**of)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s.run(**of)
+    s.seq_len.copy_(lens)
+    s.group_pages.copy_(pages)
+    graph.replay()
+    s.check(out)
+
+
 @pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.float32, 64)])
 def test_many_groups_and_the_same_result_as_row_by_row(dtype, hd):
     """Against the decode attention that reads every row's pages for itself."""

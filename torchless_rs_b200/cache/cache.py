@@ -246,10 +246,16 @@ class PagedGroup:
                 self._staging_events[self._turn].synchronize()
             stage = self._staging[self._turn]
             stage_np = stage.numpy()
-            for j, r in enumerate(rows[c0:c0 + chunk]):
-                stage_np[j] = self.table_host[r]
-                self.table_dev[r].copy_(stage[j], non_blocking=True)
-                self.bytes_copied += 4 * self.table_host.shape[1]
+            part = rows[c0:c0 + chunk]
+            stage_np[:len(part)] = self.table_host[part]
+            j = 0
+            while j < len(part):         # one copy for rows that follow one another (a reorder changes many)
+                k = j + 1
+                while k < len(part) and part[k] == part[k - 1] + 1:
+                    k += 1
+                self.table_dev[part[j]:part[k - 1] + 1].copy_(stage[j:k], non_blocking=True)
+                self.bytes_copied += 4 * self.table_host.shape[1] * (k - j)
+                j = k
             ev = self._staging_events[self._turn] or torch.cuda.Event()
             ev.record()
             self._staging_events[self._turn] = ev
@@ -276,11 +282,12 @@ class StateGroup:
     def reset(self, slot: int) -> None:
         self.storage[:, slot].zero_()
 
-    def fork(self, src: Sequence[int], dst: Sequence[int]) -> None:
-        """The state of each slot dst[i] becomes that of src[i], in all layers."""
+    def fork(self, src: Sequence[int], dst: Sequence[int], act_dtype: torch.dtype) -> None:
+        """The state of each slot dst[i] becomes that of src[i], in all layers.  `act_dtype`: whose library is loaded already (bytes
+        are copied, the state's type does not matter)."""
         if self.storage.is_cuda:
             from ..csrc import ops
-            ops.core_ops(torch.float32).copy_slots(self.storage, src, dst)     # (bytes: the state's type does not matter)
+            ops.core_ops(act_dtype).copy_slots(self.storage, src, dst)
         else:
             self.storage[:, list(dst)] = self.storage[:, list(src)]
 
@@ -425,7 +432,7 @@ class Cache:
                 g.fork(a, b)
             g.upload()
         for g in self.states:
-            g.fork(src, dst)
+            g.fork(src, dst, self.dtype)
         for a, b in zip(src, dst):
             self.lengths[b] = self.lengths[a]
 
