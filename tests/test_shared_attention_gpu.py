@@ -299,6 +299,15 @@ def test_refusals(bad):
         s.run(**change)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("name", ["q", "out"])
+def test_tensors_that_begin_inside_16_bytes_are_refused(dtype, name):
+    s = Setting(dtype, 8, 2, 64, [4, 4], [100, 300], [1, 4])
+    inside = torch.zeros(s.q.numel() + 1, dtype=dtype, device=DEV)[1:].view(s.q.shape)
+    with pytest.raises(KernelError):
+        s.run(**{name: inside})
+
+
 def test_sizes_without_a_kernel():
     assert SharedAttention.get(torch.bfloat16, 32) is None and SharedAttention.get(torch.float16, 64) is None
     assert not SharedAttention.get(torch.bfloat16, 64).takes(34, 2) and SharedAttention.get(torch.float32, 64).takes(64, 2)

@@ -614,7 +614,7 @@ extern "C" int FN(tl_attn_shared)(const void* q, const void* k_pages, const void
   if (nkv <= 0 || nh <= 0 || nh % nkv || row_blocks < 1 || parts < 2 || blocks < 1 || group_rows < 1 || window < 0) return -1;
   const int G = nh / nkv, beams = (group_rows + row_blocks - 1) / row_blocks, R = beams * G;
   if (G > SH_MAX_HEADS || R > 64 || parts > SH_MAX_PARTS || groups > SH_MAX_GROUPS || nkv > 65535 || group_rows > 65535 ||
-      n_pages * nkv * (HEAD_DIM > PAGE ? HEAD_DIM : PAGE) > 0x7fffffffLL || ((uintptr_t)q & 15) || ((uintptr_t)k_pages & 15) || ((uintptr_t)v_pages & 15))
+      n_pages * nkv * (HEAD_DIM > PAGE ? HEAD_DIM : PAGE) > 0x7fffffffLL || ((uintptr_t)q & 15) || ((uintptr_t)out & 15) || ((uintptr_t)k_pages & 15) || ((uintptr_t)v_pages & 15))
     return -2;
   CUtensorMap tk, tv;
   if (!sh_make_map(&tk, k_pages, n_pages * nkv * PAGE, HEAD_DIM, PAGE, 2)) return -2;

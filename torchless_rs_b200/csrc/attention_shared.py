@@ -125,8 +125,8 @@ class SharedAttention:
         [pages, nkv, PAGE, head_dim], `v_pages` [pages, nkv, head_dim, PAGE]).  Row r's pages are page_table[seq_slot[r]], its
         length seq_len[r].  Group g is the rows group_start[g] to group_start[g + 1] - 1, at most `group_rows` of them; they have one
         length, lens[g], and their page tables agree in the first shared[g] = group_pages[g] columns.  All of these int32 on the
-        device, `lens` and `shared` lists on the host.  `bound`: columns that common pages may come to fill while a recorded
-        graph of this call is replayed."""
+        device, `lens` and `shared` lists on the host.  `q`, `out` and the pages begin on 16-byte boundaries.  `bound`: columns that
+        common pages may come to fill while a recorded graph of this call is replayed."""
         hd, rows, groups = self.head_dim, q.shape[0], len(lens)
         if not self.takes(nh, nkv):
             raise KernelError(f"shared attention: {nh} query heads over {nkv} are not taken")

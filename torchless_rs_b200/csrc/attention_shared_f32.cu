@@ -369,7 +369,7 @@ extern "C" int tl_attn_shared_f32(const void* q, const void* k_pages, const void
   if (nkv <= 0 || nh <= 0 || nh % nkv || row_blocks < 1 || parts < 2 || blocks < 1 || group_rows < 1 || window < 0) return -1;
   const int beams = (group_rows + row_blocks - 1) / row_blocks;
   if (beams * (nh / nkv) > 32 || parts > SH_MAX_PARTS || groups > SH_MAX_GROUPS || nkv > 65535 || group_rows > 65535 ||
-      n_pages * nkv * 128 > 0x7fffffffLL || ((uintptr_t)q & 15) || ((uintptr_t)k_pages & 15) || ((uintptr_t)v_pages & 15))
+      n_pages * nkv * 128 > 0x7fffffffLL || ((uintptr_t)q & 15) || ((uintptr_t)out & 15) || ((uintptr_t)k_pages & 15) || ((uintptr_t)v_pages & 15))
     return -2;
   const ShArgs<float> a = {(const float*)q, (float*)out, part, unit_parts, seq_len, seq_slot, page_table, group_start, group_pages,
                            table_stride, groups, nh, nkv, window, scale, parts, row_blocks, beams};
