@@ -272,12 +272,12 @@ def test_forked_sequences_share_pages_and_write_their_own(requests, prompt):
     c.fork([a, a], [b, d])
     c.check()
     assert [g.pool.held_count for g in c.paged] == held and c.length(b) == c.length(d) == prompt
-    assert c.common_columns([a, b, d]) == -(-prompt // PAGE)
+    assert c.common_columns([[a, b, d]]) == [-(-prompt // PAGE)]
     _write(c, [a, b, d], [prompt + 1] * 3, [1, 2, 3])
     # the begun page was copied for two of the three; a new page where the prompt had filled its last
     for g, h in zip(c.paged, held):
         assert g.pool.held_count == h + (3 if prompt % PAGE == 0 else 2)
-    assert c.common_columns([a, b, d]) == prompt // PAGE
+    assert c.common_columns([[a, b, d]]) == [prompt // PAGE]
     for s, t in ((a, 1), (b, 2), (d, 3)):
         _expect(c, s, [(1, 0, prompt), (t, prompt, prompt + 1)])
     new = c.reorder([a, b, d], [1, 1, 0])

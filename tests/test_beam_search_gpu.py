@@ -253,6 +253,31 @@ def test_generation_after_a_search_is_what_it_was():
     assert [r.tokens for r in tm.model.generate(prompts, max_tokens=20, temperature=0.0, stop_ids=())] == want
 
 
+@pytest.mark.parametrize("slots,beams", [(5, 5), (40, 8), (100, 33)])
+def test_page_tables_reach_the_device_whichever_rows_change(slots, beams):
+    from torchless_rs_b200.cache import Cache
+    from torchless_rs_b200.cache.requests import PagedKVRequest, StateRequest
+    c = Cache([PagedKVRequest(1, 16), PagedKVRequest(1, 16, window=90), StateRequest((3,))], 64 * 20 * slots, slots, None,
+              dtype=torch.bfloat16, device=torch.device("cuda:0"))
+    rng = np.random.default_rng(slots)
+    held = np.asarray(c.acquire(slots))
+    live = sorted(rng.permutation(held)[:beams].tolist())
+    lens = [100] * beams
+    c.prepare(live, lens)
+    c.commit(live, lens)
+    for _ in range(60):
+        live = c.reorder(live, rng.integers(0, beams, beams).tolist())
+        some = sorted(rng.permutation(beams)[:max(1, int(rng.integers(beams)))].tolist())
+        lens = [c.length(s) for s in live]
+        c.prepare([live[i] for i in some], [lens[i] + 1 for i in some])
+        c.commit([live[i] for i in some], [lens[i] + 1 for i in some])
+        c.check()
+        for g in c.paged:
+            assert np.array_equal(g.table_dev.cpu().numpy(), g.table_host)
+    c.release(held.tolist())
+    c.check()
+
+
 def test_step_refuses_groups_that_do_not_fit():
     tm = TinyModel("D", "bfloat16", seed=6, max_tokens=1024)
     s = tm.engine.start_sequences(2)

@@ -118,7 +118,8 @@ class Model:
             stop_ids = self.engine.spec.stop_token_ids
 
         def select(logits, scores, n):
-            on_device = torch.tensor(scores, dtype=torch.float32).to(logits.device)
+            # (from pinned memory: the selection is enqueued behind the step, the host waits for its result only)
+            on_device = torch.tensor(scores, dtype=torch.float32, pin_memory=True).to(logits.device, non_blocking=True)
             out = self.beam_selector.ops.select(logits, on_device, n)[:3].cpu()
             return out[0].view(torch.float32), out[1], out[2]
 

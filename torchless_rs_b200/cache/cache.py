@@ -114,20 +114,24 @@ class PagedGroup:
         self._dirty.add(slot)
 
     def _drop(self, pages) -> None:
-        """One sequence less holds each of these pages; those that none holds any more go back."""
+        """One sequence less holds each of these pages (-1: none); those that none holds any more go back."""
         pages = [int(p) for p in pages if p >= 0]
         self.holders[pages] -= 1
         self.pool.give_back(p for p in pages if self.holders[p] == 0)
 
-    def fork(self, src: int, dst: int) -> None:
-        """The slot `dst` lets go of what it holds and holds the pages of `src` from now on."""
-        c = self.n_cols[dst]
-        self._drop(self.table_host[dst, :c])
+    def fork(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Each slot dst[i] lets go of what it holds and holds the pages of src[i] from now on."""
+        cols = max(self.n_cols[s] for s in dst)
+        gone = self.table_host[dst, :cols].ravel()
+        gone = gone[gone >= 0]
+        np.subtract.at(self.holders, gone, 1)
+        held = self.table_host[src, :max(self.n_cols[s] for s in src)]
         self.table_host[dst] = self.table_host[src]
-        held = self.table_host[src, :self.n_cols[src]]
-        self.holders[held[held >= 0]] += 1
-        self.first_live[dst], self.n_cols[dst] = self.first_live[src], self.n_cols[src]
-        self._dirty.add(dst)
+        np.add.at(self.holders, held[held >= 0], 1)
+        self.pool.give_back(np.unique(gone[self.holders[gone] == 0]).tolist())
+        for a, b in zip(src, dst):
+            self.first_live[b], self.n_cols[b] = self.first_live[a], self.n_cols[a]
+        self._dirty.update(dst)
 
     def writes_into_shared(self, slots: Sequence[int], lengths: Sequence[int]) -> List[int]:
         """Which of `slots` (indices into the list) need a page of their own before they write position lengths[i]: their last page is
@@ -175,11 +179,15 @@ class PagedGroup:
                     view.k_pages[b, :, :c] = view.k_pages[a, :, :c]
                     view.v_pages[b, :, :, :c] = view.v_pages[a, :, :, :c]
 
-    def common_columns(self, slots: Sequence[int]) -> int:
-        """The leading columns in which the tables of `slots` agree."""
-        rows = self.table_host[list(slots), :max(self.n_cols[s] for s in slots)]
-        differ = np.flatnonzero((rows != rows[0]).any(axis=0))
-        return int(differ[0]) if len(differ) else rows.shape[1]
+    def common_columns(self, groups: Sequence[Sequence[int]]) -> np.ndarray:
+        """Per group of slots (all of one size) the leading columns in which their tables agree."""
+        slots = np.asarray(groups)
+        cols = np.asarray([max(self.n_cols[s] for s in g) for g in groups])
+        width = int(cols.max())
+        rows = self.table_host[slots, :width]                     # [groups, slots, columns]
+        differ = np.ones((len(groups), width + 1), dtype=bool)    # (the column behind the last one ends what they have in common)
+        differ[:, :width] = (rows != rows[:, :1]).any(axis=1)
+        return np.minimum(differ.argmax(axis=1), cols)
 
     def trim(self, slot: int, next_pos: int) -> None:
         """Gives back the pages that no position >= next_pos can see any more."""
@@ -236,26 +244,34 @@ class PagedGroup:
             self.table_dev.index_copy_(0, idx, torch.from_numpy(self.table_host[rows]))
             return
         chunk = 32   # rows per snapshot buffer
+        width = self.table_host.shape[1]
         if self._staging is None:
-            self._staging = torch.empty((4, chunk, self.table_host.shape[1]), dtype=torch.int32,
-                                        pin_memory=True)
+            self._staging = torch.empty((4, chunk, width), dtype=torch.int32, pin_memory=True)
             self._staging_events = [None] * 4
-        for c0 in range(0, len(rows), chunk):
+        # One copy for dirty rows that lie close together, with those between (a reorder changes many rows, and a copy costs more than
+        # 8 KB of it): [first, last] pairs, at most `chunk` rows long.
+        spans: List[List[int]] = []
+        for r in rows:
+            if spans and r - spans[-1][0] < chunk and (r == spans[-1][1] + 1 or (len(rows) > 2 and (r - spans[-1][1] - 1) * width <= 2048)):
+                spans[-1][1] = r
+            else:
+                spans.append([r, r])
+        i = 0
+        while i < len(spans):
             self._turn = (self._turn + 1) % 4
             if self._staging_events[self._turn] is not None:
                 self._staging_events[self._turn].synchronize()
             stage = self._staging[self._turn]
             stage_np = stage.numpy()
-            part = rows[c0:c0 + chunk]
-            stage_np[:len(part)] = self.table_host[part]
-            j = 0
-            while j < len(part):         # one copy for rows that follow one another (a reorder changes many)
-                k = j + 1
-                while k < len(part) and part[k] == part[k - 1] + 1:
-                    k += 1
-                self.table_dev[part[j]:part[k - 1] + 1].copy_(stage[j:k], non_blocking=True)
-                self.bytes_copied += 4 * self.table_host.shape[1] * (k - j)
-                j = k
+            at = 0
+            while i < len(spans) and at + spans[i][1] - spans[i][0] < chunk:
+                first, end = spans[i][0], spans[i][1] + 1
+                n = end - first
+                stage_np[at:at + n] = self.table_host[first:end]
+                self.table_dev[first:end].copy_(stage[at:at + n], non_blocking=True)
+                self.bytes_copied += 4 * width * n
+                at += n
+                i += 1
             ev = self._staging_events[self._turn] or torch.cuda.Event()
             ev.record()
             self._staging_events[self._turn] = ev
@@ -428,8 +444,7 @@ class Cache:
         if not src:
             return
         for g in self.paged:
-            for a, b in zip(src, dst):
-                g.fork(a, b)
+            g.fork(src, dst)
             g.upload()
         for g in self.states:
             g.fork(src, dst, self.dtype)
@@ -459,9 +474,11 @@ class Cache:
         self.fork(src, dst)
         return out
 
-    def common_columns(self, slots: Sequence[int]) -> int:
-        """The leading pages that the sequences of `slots` hold together, in every group of layers."""
-        return min((g.common_columns(slots) for g in self.paged), default=0)
+    def common_columns(self, groups: Sequence[Sequence[int]]) -> List[int]:
+        """Per group of slots (all of one size) the leading pages that their sequences hold together, in all layers."""
+        if not self.paged or not groups:
+            return [0] * len(groups)
+        return np.minimum.reduce([g.common_columns(groups) for g in self.paged]).tolist()
 
     # ---- one step ----------------------------------------------------------------
     def prepare(self, slots: Sequence[int], new_lens: Sequence[int]) -> None:

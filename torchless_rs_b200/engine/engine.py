@@ -188,15 +188,20 @@ class Engine:
         if groups is None:
             return None
         rows, lens, shared = [], [], []
-        at = 0
+        starts = [0]
         for n in groups:
-            ss, ls = slots[at:at + n], new_lens[at:at + n]
-            at += n
-            common = self.cache.common_columns(ss) if n > 1 and len(set(ls)) == 1 else 0
-            if common:
+            starts.append(starts[-1] + n)
+        common = [0] * len(groups)
+        for n in set(groups) - {1}:
+            those = [i for i, m in enumerate(groups) if m == n and len(set(new_lens[starts[i]:starts[i + 1]])) == 1]
+            for i, c in zip(those, self.cache.common_columns([slots[starts[i]:starts[i + 1]] for i in those])):
+                common[i] = c
+        for i, n in enumerate(groups):
+            ls = new_lens[starts[i]:starts[i + 1]]
+            if common[i]:
                 rows.append(n)
                 lens.append(ls[0])
-                shared.append(common)
+                shared.append(common[i])
             else:                      # rows by themselves
                 rows += [1] * n
                 lens += list(ls)
