@@ -159,6 +159,48 @@ def test_scores_that_grow_from_page_to_page(dtype, nh, nkv, hd):
         s.check()
 
 
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS + [(torch.bfloat16, 16, 1, 64), (torch.bfloat16, 16, 1, 128)])
+@pytest.mark.parametrize("blocks", [1, 3])
+@pytest.mark.parametrize("step", [3.0, 10.0, 20.0, 45.0, -10.0, -45.0])
+def test_scores_that_grow_within_a_block(dtype, nh, nkv, hd, blocks, step, monkeypatch):
+    """The same where one block sees many pages one after the other: references move, or weights leave their range."""
+    from torchless_rs_b200.csrc import attention_shared
+    monkeypatch.setattr(attention_shared, "_sm_count", lambda device: blocks)
+    s = Setting(dtype, nh, nkv, hd, [4, 2], [1500, 200], [20, 1], seed=2)
+    q = s.q.view(-1, nh, hd)
+    q[:, :, 0] = 1.0
+    q[1, :, 0] = -1.0
+    q[2, 0, 0] = 0.0
+    s.k[:, :, :, 0] = 0.0
+    for row in s.table:
+        for c, page in enumerate(row):
+            if page >= 0:
+                s.k[page, :, :, 0] = c * step / s.scale
+    s.check()
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("blocks", [1, 148])
+@pytest.mark.parametrize("far", [30.0, 70.0, 100.0, 300.0, -30.0, -100.0, float("nan"), float("inf"), float("-inf")])
+def test_a_first_key_that_stands_out_in_pages_of_another_row(dtype, nh, nkv, hd, blocks, far, monkeypatch):
+    """No common pages: the first key that a block sees is row 0's own, and lies far from what the other rows see."""
+    from torchless_rs_b200.csrc import attention_shared
+    monkeypatch.setattr(attention_shared, "_sm_count", lambda device: blocks)
+    s = Setting(dtype, nh, nkv, hd, [4], [150], [0], seed=6)
+    q = s.q.view(-1, nh, hd)
+    q[:, :, 0] = 1.0
+    s.k[:, :, :, 0] = 0.0
+    s.k[s.table[0][0], :, 0, 0] = far / s.scale
+    if math.isfinite(far):
+        s.check()
+        return
+    got = s.run().view(4, nh, hd)
+    want, mass = s.plain()
+    assert torch.isfinite(got[1:]).all()
+    bound = (mass * 2.0 ** -8 * 1.1 + want.abs() * 2.0 ** -8).view(4, nh, hd)[1:]
+    assert ((got[1:].double() - want.view(4, nh, hd)[1:]).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
 def test_scores_far_apart_and_scale(dtype, nh, nkv, hd):
     s = Setting(dtype, nh, nkv, hd, [4, 2], [700, 90], [9, 1], spread=0.2, seed=1)

@@ -9,8 +9,8 @@
 // N = 16, 32 or 64; more rows take several units) against the shared pages and then each row's own.  On the fifth-generation
 // tensor cores keys take the 128 lanes and rows the columns, so that few rows cost little:
 //   S^T[128 keys, N]  = K . Q^T      two pages of keys, Q in shared memory, S^T in tensor memory (two buffers)
-//   softmax           a key and half of the columns per thread; a column's reference is the score of the first key that it sees and
-//                     moves only when another exceeds it by 2^60, so that a tile needs one barrier of four warps and no maxima; P^T
+//   softmax           a key and half of the columns per thread; a column's reference is the score of the first key of the stretch and
+//                     moves only when another exceeds it by 2^60, so that a tile needs no barrier and no maxima; P^T
 //                     rounded to bfloat16 (by at most 2^-8 of each weight: the products take bfloat16) to shared memory
 //   O^T[hd, N]       += V^T . P^T    the transposed value slab as it lies in the cache, O^T in tensor memory
 // A row's own page is multiplied with all rows of the unit; the others' weights are zero there, as all weights of keys that are not seen
@@ -45,9 +45,11 @@
 #define SH_PAGE_V (HEAD_DIM * PAGE * 2)
 #define SH_STRIDE (HEAD_DIM + 2)                    // floats of a partial result: weighted sum, maximum, sum
 #define SH_MAX_HEADS 16                             // query heads per key/value head
-// A column's reference is the score of the first key that it sees and moves when a score exceeds it by 2^60: weights of up to that,
-// their sums and products with values are far from 32 bits' ends, and rounding to bfloat16 is relative.
+// A column's reference moves two tiles after a score has exceeded it by 2^60 (in between weights reach what the two tiles' scores exceed it
+// by; at 2^127 the result is none and is computed again), so that no tile waits for a maximum; rounding to bfloat16 is relative.  A sum of
+// weights below 2^-60 is not taken either: what is lost below 2^-126 is then no more than 2^-66 of it.
 #define SH_SLACK 60.0f
+#define SH_LEAST 8.67361737988403547e-19f            // 2^-60
 
 __device__ int tl_attn_shared_error = 0;
 
@@ -62,7 +64,6 @@ __device__ __forceinline__ float sh_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void sh_bar(int half) { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); }   // four softmax warps
 __device__ __forceinline__ void sh_async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // C columns of this thread's lane: 8 at a time
 template <int C>
@@ -153,7 +154,7 @@ template <int N>
 struct ShSizes {
   static constexpr int KS = HEAD_DIM == 64 ? (N == 64 ? 4 : 6) : (N == 64 ? 2 : 3), VS = HEAD_DIM == 64 ? 4 : 2;   // ring slots of two pages
   static constexpr int K = 2 * SH_PAGE_K, V = 2 * SH_PAGE_V, Q = N * HEAD_DIM * 2, P = 2 * N * 128;
-  static constexpr int aux = SH_MAX_GROUPS * (int)sizeof(ShGroup) + 9 * N * 4 + 512;
+  static constexpr int aux = SH_MAX_GROUPS * (int)sizeof(ShGroup) + 7 * N * 4 + 512;
   static constexpr int smem = KS * K + VS * V + 2 * Q + 2 * P + aux;
   static constexpr uint32_t tmem = N == 16 ? 64 : N == 32 ? 128 : 256;                             // S^T twice, O^T
 };
@@ -170,9 +171,8 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   uint8_t* p_s = q_s + 2 * Z::Q;                       // [2][P]
   ShGroup* table = (ShGroup*)(p_s + 2 * Z::P);
   float* red_s = (float*)(table + SH_MAX_GROUPS);      // [4][N]
-  float* new_s = red_s + 4 * N;                        // [2][N]: scores of the first keys that columns see, by page of the tile
-  float* ref_s = new_s + 2 * N;                        // [N]
-  float* neg_s = ref_s + N;                            // [N]: the negated references, 0 for a column that has none
+  float* ref_s = red_s + 4 * N;                        // [N]
+  float* neg_s = ref_s + N;                            // [N]: the negated references
   float* al_s = neg_s + N;                             // [N]
   uint64_t* k_full = (uint64_t*)(al_s + N);
   uint64_t* k_empty = k_full + Z::KS;
@@ -183,13 +183,15 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   uint64_t* pv_done = p_full + 2;                      // [2]
   uint64_t* q_full = pv_done + 2;                      // [2]
   uint64_t* o_free = q_full + 2;
-  uint32_t* tmem_slot = (uint32_t*)(o_free + 1);
+  uint64_t* half_bar = o_free + 1;                     // [2]
+  uint32_t* tmem_slot = (uint32_t*)(half_bar + 2);
   int* total_s = (int*)(tmem_slot + 1);                // [3]
   volatile int* abort_flag = (volatile int*)(total_s + 3);
-  // [2][3]: a reference in this half of the columns has to move.  By tile number modulo 3: written before a tile's barrier, read after
-  // it, cleared behind the next one (what a warp that runs ahead writes by then is another tile's).
+  // [2][8]: a reference in this half of the columns has to move.  By tile number modulo 8: written in tile n, read in tile n + 2 when
+  // its wait has shown that every warp is through with tile n, cleared in tile n + 6 (then every warp has read it, and none is as far
+  // as tile n + 8).
   volatile int* moved_s = abort_flag + 1;
-  ShPiece* first_s = (ShPiece*)(abort_flag + 1 + 6);   // the stretch's first unit
+  ShPiece* first_s = (ShPiece*)(abort_flag + 1 + 16);   // the stretch's first unit
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (smem_u32(sh_smem) & 1023u) {                     // nothing has been allocated yet
@@ -204,8 +206,9 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       mbar_init(&p_full[u], SH_SOFT);
       mbar_init(&pv_done[u], 1);
       mbar_init(&q_full[u], SH_SOFT);
+      mbar_init(&half_bar[u], SH_SOFT / 2);
     }
-    for (int u = 0; u < 6; ++u) moved_s[u] = 0;
+    for (int u = 0; u < 16; ++u) moved_s[u] = 0;
     mbar_init(o_free, SH_SOFT);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -376,12 +379,18 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         }
       }
     } else if (warp < 8) {
-      // ---- softmax: key `key` of a tile, columns first_col to first_col + NC - 1.  A wait that runs out leaves the loop's barriers in
-      // place: the warps go through them to the end (every later wait returns at once), and what they write is not valid.
+      // ---- softmax: key `key` of a tile, columns first_col to first_col + NC - 1.  After a wait that runs out the warps go through the loop
+      // to the end (every later wait returns at once), and what they write is not valid.
       constexpr int NC = N / 2;
       const int upper = warp >> 2, key = tid & 127, page_of = key >> 6, first_col = upper * NC, quad = warp & 3;
       const uint32_t t_lane = (uint32_t)(quad * 32) << 16;
-      volatile int* moved = moved_s + 3 * upper;
+      volatile int* moved = moved_s + 8 * upper;
+      uint32_t met_before = 0;
+      auto meet = [&] {                        // the four warps of this half, by a wait that is bounded too
+        sh_arrive(&half_bar[upper]);
+        sh_park(&half_bar[upper], met_before, abort_flag, 14);
+        met_before ^= 1u;
+      };
       const int my_col = first_col + (key & (NC - 1)), my_beam = my_col / G, my_head = my_col - my_beam * G;
       const int first_beam = first_col / G, first_head = first_col - first_beam * G;
       const ShRow q_row(tid / (HEAD_DIM / 8), G);
@@ -417,42 +426,22 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         ShPiece np = {};
 #pragma unroll
         for (int c = 0; c < NC; ++c) l[c] = 0.0f;
-        if (key < NC) {
-          ref_s[first_col + key] = -INFINITY;
-          neg_s[first_col + key] = 0.0f;
-        }
-        sh_bar(upper);
         const uint32_t all = sh_mask(0, min(max(R - first_col, 0), NC));
-        uint32_t is_set = 0;                   // columns that have a reference
-        // the tile's two pages, step by step
-        struct { int owner, in_own, col; } page[2];
-        page[0] = {-1, 0, p.first + 2 * p.tile};
-        if (2 * p.tile >= p.common) {
-          page[0].owner = p.own ? (2 * p.tile - p.common) / p.own : 0;
-          page[0].in_own = 2 * p.tile - p.common - page[0].owner * p.own;
-          page[0].col = p.first + p.common + page[0].in_own;
-        }
-        auto step = [&](int to, int from) {
-          int owner = page[from].owner, in_own = page[from].in_own, col = page[from].col + 1;
-          if (owner < 0) {
-            if (col == p.first + p.common) owner = 0;
-          } else if (++in_own >= p.own) {
-            in_own = 0;
-            ++owner;
-            col = p.first + p.common;
-          }
-          page[to] = {owner, in_own, col};
-        };
-        step(1, 0);
-        // the columns that see a page, of this half
+        // the columns of this half that see a page
         auto seen_by = [&](int owner) {
           return owner < 0 ? all : sh_mask(min(max(owner * G - first_col, 0), NC), min(max(owner * G + G - first_col, 0), NC));
         };
+        // this thread's page of the tile, step by step
+        int owner = -1, in_own = 0, col = p.first + 2 * p.tile + page_of;
+        if (2 * p.tile + page_of >= p.common) {
+          owner = p.own ? (2 * p.tile + page_of - p.common) / p.own : 0;
+          in_own = 2 * p.tile + page_of - p.common - owner * p.own;
+          col = p.first + p.common + in_own;
+        }
+        uint32_t columns = seen_by(owner);
         for (int j = p.tile; j < last; ++j, ++n) {
-          const int buf = n & 1, now3 = n % 3;
+          const int buf = n & 1;
           const bool there = 2 * j + page_of < p.pages;
-          const int owner = page_of ? page[1].owner : page[0].owner, col = page_of ? page[1].col : page[0].col;
-          const uint32_t columns = seen_by(owner);
           const int at = col * PAGE + (key & 63);
           const bool seen = there && at >= p.lo && at < p.len;
           const bool plain = there && owner < 0 && col * PAGE >= p.lo && col * PAGE + PAGE <= p.len;
@@ -461,52 +450,42 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           float s[NC];                         // scores, then weights
           const uint32_t t_s = tmem + t_lane + (uint32_t)buf * N + first_col;
           sh_tmem_ld<NC>(t_s, s);
-          if (is_set != all) {
-            // columns that see their first keys: the score of the first of them becomes the reference
-            uint32_t of[2] = {0u, 0u};
+          if (j == p.tile) {
+            // The references: every column's score of the first key that the tile has to see, whoever sees it.  (A row's own keys may lie far
+            // from it: where its weights come to nothing, its result is computed again.)
+            if (key == max(p.lo - col * PAGE, 0)) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (2 * j + h >= p.pages) continue;
-              of[h] = seen_by(page[h].owner) & ~is_set;
-              if (of[h] && key == h * PAGE + max(p.lo - page[h].col * PAGE, 0)) {
+              for (int c = 0; c < NC; c += 4) {
+                float r[4];
 #pragma unroll
-                for (int c = 0; c < NC; c += 4)
-                  *reinterpret_cast<float4*>(new_s + h * N + first_col + c) = make_float4(s[c], s[c + 1], s[c + 2], s[c + 3]);
+                for (int e = 0; e < 4; ++e) r[e] = fminf(fmaxf(s[c + e] * a.scale, -1e30f), 1e30f);       // (no number: -1e30)
+                *reinterpret_cast<float4*>(ref_s + first_col + c) = make_float4(r[0], r[1], r[2], r[3]);
+                *reinterpret_cast<float4*>(neg_s + first_col + c) = make_float4(-r[0], -r[1], -r[2], -r[3]);
               }
             }
-            of[1] &= ~of[0];
-            if (of[0] | of[1]) {
-              sh_bar(upper);
-              if (key < NC && (of[0] | of[1]) >> key & 1u) {
-                const float first = new_s[((of[0] >> key & 1u) ? 0 : N) + first_col + key];
-                const float ref = fmaxf(first * a.scale, -1e30f);
-                ref_s[first_col + key] = ref;
-                neg_s[first_col + key] = -ref;
-              }
-              sh_bar(upper);
-              is_set |= of[0] | of[1];
-            }
+            meet();
           }
           const float largest = plain ? sh_shift<false>(s, columns, neg, a.scale) : sh_shift<true>(s, seen ? columns : 0u, neg, a.scale);
-          if (__any_sync(0xffffffffu, largest > SH_SLACK) && lane == 0) moved[now3] = 1;
-          sh_bar(upper);
-          if (key == 0) moved[(n + 2) % 3] = 0;
-          if (moved[now3]) {
+          // (These scores were issued after the product with P^T of two tiles ago and are done after it: its buffer is free, and every warp is
+          // through with that tile, so they agree on what it noted.)
+          if (__any_sync(0xffffffffu, largest > SH_SLACK) && lane == 0) moved[n & 7] = 1;
+          if (key == 0) moved[(n + 2) & 7] = 0;
+          if (n >= 2 && moved[(n - 2) & 7]) {
             // another reference for the columns that need one: the maximum of this tile's scores
             sh_tmem_ld<NC>(t_s, s);
 #pragma unroll
             for (int c = 0; c < NC; ++c) s[c] = seen && (columns >> c & 1u) ? s[c] * a.scale : -INFINITY;
             sh_columns<NC>(s, lane, red_s + quad * N + first_col, [](float x, float y) { return fmaxf(x, y); });
-            sh_bar(upper);
+            meet();
             if (key < NC) {
               const float* r = red_s + first_col + key;
               const float m = fmaxf(fmaxf(r[0], r[N]), fmaxf(r[2 * N], r[3 * N])), old = ref_s[first_col + key];
               const float now = m > old + SH_SLACK ? m : old;
               ref_s[first_col + key] = now;
-              neg_s[first_col + key] = now == -INFINITY ? 0.0f : -now;
+              neg_s[first_col + key] = -now;
               al_s[first_col + key] = now == old ? 1.0f : sh_ex2(old - now);
             }
-            sh_bar(upper);
+            meet();
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
               l[c] *= al_s[first_col + c];
@@ -525,8 +504,7 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
               sh_tmem_st_wait();
             }
           }
-          // weights; P^T of two tiles ago has been read
-          if (n >= 2) sh_park(&pv_done[buf], (uint32_t)((n - 2) >> 1) & 1u, abort_flag, 11);
+          // weights
           const uint32_t pw = smem_u32(p_s + buf * Z::P + page_of * (N * 128) + first_col * 128), k2 = (uint32_t)(key & 63) * 2;
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
@@ -543,12 +521,24 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
             np = piece(p.next);
             if (np.tile < np.last) load_q(np, (unit + 1) & 1);
           }
-          step(0, 1);
-          step(1, 0);
+          // two pages on
+          const int before = owner;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            ++col;
+            if (owner < 0) {
+              if (col == p.first + p.common) owner = 0;
+            } else if (++in_own >= p.own) {
+              in_own = 0;
+              ++owner;
+              col = p.first + p.common;
+            }
+          }
+          if (owner != before) columns = seen_by(owner);
         }
         // ---- the unit's end: sums over the keys, O^T out
         sh_columns<NC>(l, lane, red_s + quad * N + first_col, [](float x, float y) { return x + y; });
-        sh_bar(upper);
+        meet();
         const int first_block = p.start / share, pieces = (p.start + p.tiles - 1) / share - first_block + 1;
         const int slot = (int)blockIdx.x - first_block;
         if (tid == 0 && slot == 0) a.unit_parts[p.unit] = pieces;
@@ -556,8 +546,12 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         const int heads = a.parts * SH_STRIDE;
         if (key < NC && my_col < R) {
           float* dst = a.part + ((size_t)(p.row0 + my_beam) * a.nh + p.kvh * G + my_head) * heads + slot * SH_STRIDE + HEAD_DIM;
-          dst[0] = ref_s[my_col];
-          dst[1] = (red_s[my_col] + red_s[N + my_col]) + (red_s[2 * N + my_col] + red_s[3 * N + my_col]);
+          const float sum = (red_s[my_col] + red_s[N + my_col]) + (red_s[2 * N + my_col] + red_s[3 * N + my_col]);
+          // (the columns that have seen a key: all, or those of the rows whose own pages these were)
+          const int from = 2 * p.tile - p.common, to = min(2 * last, p.pages) - 1 - p.common;
+          const bool any = from < 0 || (my_beam >= from / p.own && my_beam <= to / p.own);
+          dst[0] = any ? ref_s[my_col] : -INFINITY;
+          dst[1] = any && !(sum >= SH_LEAST) ? NAN : sum;       // (too little of it is left)
         }
         sh_park(&pv_done[(n - 1) & 1], (uint32_t)((n - 1) >> 1) & 1u, abort_flag, 13);
         tc_fence_after();
@@ -579,7 +573,7 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         }
         tc_fence_before();
         sh_arrive(o_free);
-        sh_bar(upper);                         // red_s and ref_s are written again
+        meet();                         // red_s and ref_s are written again
         p = np;
       }
     }
