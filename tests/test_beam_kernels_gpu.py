@@ -72,6 +72,18 @@ def test_select(S, B, V, n, spread):
     _check_select(*_rand(rng, S, B, V, spread), n)
 
 
+@pytest.mark.parametrize("S,B,V,n", [(1, 64, 2000, 128), (2, 32, 9000, 64), (1, 16, 40000, 32), (3, 40, 5000, 100), (1, 100, 300, 128),
+                                     (1, 8, 140000, 128)])
+@pytest.mark.parametrize("dead", [0, 1])
+def test_select_of_more_candidates_than_threads_hold(S, B, V, n, dead):
+    """Beams whose candidates are many, some beams without a score; all of one row above the others' too."""
+    logits, scores = _rand(np.random.default_rng(S + B + V), S, B, V)
+    if dead:
+        scores[:, ::3] = -np.inf
+        scores[:, 1] += 50.0
+    _check_select(logits, scores, n)
+
+
 @pytest.mark.parametrize("V", [7, 600, 9000, 40000])
 def test_select_ties_go_to_the_lowest_beam_and_token(V):
     rng = np.random.default_rng(V)

@@ -372,7 +372,6 @@ beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ can
   __shared__ BsCand gm[GROUPS];
   __shared__ BsCand buf[BS_CAP];
   __shared__ BsCand bound;
-  __shared__ BsCand wbest[BS_THREADS / 32];
   __shared__ int count;
   const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t row0 = (size_t)s * B;
@@ -454,20 +453,33 @@ beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ can
     if (rank == (n < GROUPS ? n : GROUPS) - 1) bound = of;
   }
   __syncthreads();
-  const BsCand bd = bound;
+  BsCand bd = bound;
   auto collect = [&](const BsCand& e) {
     if (e.at != 0xffffffffu && !bs_before(bd, e)) {
       const int at = atomicAdd(&count, 1);
       if (at < BS_CAP) buf[at] = e;
     }
   };
-  if (CAND) {
+  if (CAND) {                             // (held candidates are at most as many as there is room for)
 #pragma unroll
     for (int j = 0; j < HELD; ++j) collect(mine[j]);
+    __syncthreads();
   } else {
-    for (int i = tid; i < total; i += BS_THREADS) collect(value(raw(i)));
+    for (;;) {
+      for (int i = tid; i < total; i += BS_THREADS) collect(value(raw(i)));
+      __syncthreads();
+      if (count <= BS_CAP) break;
+      // more reach the bound than there is room for: the n-th of those collected is the next one (which leaves out all but n of them)
+      for (int i = tid; i < BS_CAP; i += BS_THREADS) {
+        const BsCand e = buf[i];
+        if (bs_rank(buf, BS_CAP, e) == n - 1) bound = e;
+      }
+      __syncthreads();
+      bd = bound;
+      if (tid == 0) count = 0;
+      __syncthreads();
+    }
   }
-  __syncthreads();
   const int c = count;
   const size_t o0 = (size_t)s * n;
   auto put = [&](int r, const BsCand& e) {
@@ -478,39 +490,14 @@ beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ can
     beams[o0 + r] = got ? (int)beam : -1;
     tokens[o0 + r] = got ? (int)(e.at - beam * (uint32_t)V) : -1;
   };
-  if (CAND || c <= BS_CAP) {              // (held candidates are at most as many as there is room for)
-    for (int i = tid; i < max(c, n); i += BS_THREADS) {
-      BsCand e = none;
-      int rank = i;                       // places without a candidate
-      if (i < c) {
-        e = buf[i];
-        rank = bs_rank(buf, c, e);
-      }
-      if (rank < n) put(rank, e);
+  for (int i = tid; i < max(c, n); i += BS_THREADS) {
+    BsCand e = none;
+    int rank = i;                         // places without a candidate
+    if (i < c) {
+      e = buf[i];
+      rank = bs_rank(buf, c, e);
     }
-  } else {
-    // more reach the bound than there is room for (they bunch in few threads): one after the other
-    BsCand last = {~0ull, 0u};
-    for (int r = 0; r < n; ++r) {
-      BsCand m = none;
-      for (int i = tid; i < total; i += BS_THREADS) {
-        const BsCand e = value(raw(i));
-        if (e.at != 0xffffffffu && (r == 0 || bs_before(last, e)) && bs_before(e, m)) m = e;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const BsCand other = bs_shfl(m, o);
-        if (bs_before(other, m)) m = other;
-      }
-      if (lane == 0) wbest[warp] = m;
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < BS_THREADS / 32; ++k)
-        if (bs_before(wbest[k], m)) m = wbest[k];
-      __syncthreads();
-      last = m;
-      if (tid == 0) put(r, m);
-    }
+    if (rank < n) put(rank, e);
   }
 }
 
@@ -531,7 +518,14 @@ extern "C" long long tl_beam_scratch_bytes(int rows, int V, int n) {
 template <int GS>
 static int bs_run(const float* logits, long long ld, int S, int B, int V, const float* scores, int n, void* scratch, float* values,
                   int* beams, int* tokens, cudaStream_t stream) {
-  const int rows = S * B, chunk = bs_chunk(rows, V), parts = bs_parts(V, chunk, ld % 4 != 0 || ((uintptr_t)logits & 15));
+  const bool shifted = ld % 4 != 0 || ((uintptr_t)logits & 15);
+  const int rows = S * B;
+  int chunk = bs_chunk(rows, V);
+  // Longer parts where they leave no more candidates than the second kernel's threads hold: one sequence of 8 beams, 16 continuations, 262144
+  // entries: parts of one tile 33 us, of 8 tiles 19 us; 16 beams, 32 continuations, 131072 entries 146 and 33.  (More than 8
+  // tiles gain no more.)
+  while ((long long)B * bs_parts(V, chunk, shifted) * n > 4 * BS_THREADS && chunk < 8 * BS_TILE && chunk < V) chunk *= 2;
+  const int parts = bs_parts(V, chunk, shifted);
   BsPart* part = (BsPart*)scratch;
   uint2* cand = (uint2*)(part + (size_t)rows * parts);
   const int st = tl_launch(beam_rows_kernel<GS>, dim3(parts, rows), dim3(BS_THREADS), 0, stream, logits, ld, V, scores, n, chunk, part, cand);
