@@ -135,6 +135,24 @@ def test_select_entries_that_bunch_in_few_groups(V, n):
     _check_select(y, (-rng.random((16, 4))).astype(np.float32), n)
 
 
+@pytest.mark.parametrize("V,n", [(5000, 16), (40000, 8), (140000, 16), (140000, 100)])
+@pytest.mark.parametrize("order", ["rising", "falling", "the largest at the end", "the largest at the end, and NaN", "one value"])
+def test_select_entries_in_an_order(V, n, order):
+    rng = np.random.default_rng(V + n)
+    logits, scores = _rand(rng, 2, 3, V)
+    if order in ("rising", "falling"):
+        logits.sort(axis=1)
+        if order == "falling":
+            logits = np.ascontiguousarray(logits[:, ::-1])
+    elif order == "one value":
+        logits[:] = 0.5
+    else:
+        logits[:, -3000:] += 30.0
+        if "NaN" in order:
+            logits[:, V // 2::97] = np.nan
+    _check_select(logits, scores, n)
+
+
 def test_select_peaked_rows_and_near_ties():
     """One entry holds nearly all weight, and candidates of other beams come within 1e-6 of each other."""
     rng = np.random.default_rng(5)
