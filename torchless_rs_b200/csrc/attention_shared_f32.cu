@@ -9,9 +9,10 @@
 // 1.1 us at the SM's full rate, 32 rows 2.1 us.  Pages come by TMA, keys in boxes of 32 dimensions and values in boxes of 32 keys,
 // whose 128-byte swizzle keeps the reads of neighbouring rows in different banks.  Two blocks share an SM (one's barriers and
 // softmax under the other's products); the next page's keys are requested when the scores are done, its values after the products.
-// Measured: 4 prompts of 500 to 2000 tokens x 4 beams, 32 over 8 heads of 128, 51 MB: 30 us; an SM issues 1.8 instructions a cycle of 4, 59 % of
-// them multiply-adds (eight warps of 128 registers do not hide the reads of shared memory and the four barriers of a page).  One
-// block per SM with two buffers for pages: 35 us.
+// Measured: 4 prompts of 500 to 2000 tokens x 4 beams, 32 over 8 heads of 128, 51 MB: 30 us.  A page takes 13900 instructions of a warp, 8200 of
+// them multiply-adds; the busiest SM issues 62 % of what it could (eight warps of 128 registers do not hide the reads of shared memory
+// and the four barriers of a page), and it has a third more pages than the mean, since pages are dealt whole.  One block per SM with two
+// buffers for pages: 35 us.  Weights against a reference instead of maxima (a barrier less), stretches that differ by a page at most: 29.5 to 30 us.
 //
 // Nothing is read before the wait for the kernels before: a page may have been copied by one of them.  Every wait on an mbarrier
 // is bounded; when a bound is hit the block records a code in tl_attn_shared_f32_error, waits (bounded) for its copies in flight and returns.
