@@ -245,6 +245,18 @@ def test_rows_of_length_zero_give_zero(dtype, nh, nkv, hd):
 
 
 @pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+def test_rows_behind_the_last_group_and_groups_without_rows(dtype, nh, nkv, hd):
+    s = Setting(dtype, nh, nkv, hd, [3, 2], [200, 330], [3, 4], seed=11)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    q = torch.cat([s.q, s.q[:2] * float("nan")])
+    out = torch.full_like(q, 7.0)
+    s.run(q=q, out=out, seq_len=i32(s.row_len + [10 ** 6, -1]), seq_slot=i32(s.seq_slot.tolist() + [10 ** 6, -5]),
+          group_start=i32([0, 0, 3, 3, 5, 5]), group_pages=i32([0, 3, 100, 4, 0]), lens=[440, 200, 0, 330, 64], shared=[0, 3, 0, 4, 0])
+    s.check(out[:5])
+    assert (out[5:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
 def test_every_way_of_cutting_gives_the_result(dtype, nh, nkv, hd, monkeypatch):
     from torchless_rs_b200.csrc import attention_shared
     s = Setting(dtype, nh, nkv, hd, [4, 3], [1000, 333], [12, 3], seed=8)
