@@ -102,6 +102,7 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, int V, const fl
   __shared__ u64 bound;
   __shared__ u64 wmax[BS_THREADS / 32];
   __shared__ double wsum[BS_THREADS / 32];
+  __shared__ u64 wfixed[BS_THREADS / 32];
   __shared__ int count;
   pdl_wait();
   pdl_launch_dependents();
@@ -323,16 +324,22 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, int V, const fl
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
+  // The collected ones lie in no particular order: they are added as whole multiples of 2^-52, so that the sum does not depend on it (at
+  // most 1024 of at most 1).  (Lane 0 of a warp has the warp's rest beside its entries.)
   double sum = 0.0;
-  // (lane 0 of a warp has the warp's rest beside its entries)
+  u64 fixed = 0;
   for (int i = lane == 0 ? tid - BS_THREADS : tid; i < c; i += BS_THREADS) {
-    const double weight = i < 0 ? rest : 1.0;
     const double at = i < 0 ? (double)ref : (double)bs_value((uint32_t)(buf[i] >> 32));
-    if (weight != 0.0) sum += weight * exp(at - (double)M);
+    if (i < 0 && rest == 0.0) continue;
+    const double e = exp(at - (double)M);
+    if (i < 0) sum = rest * e; else fixed += (u64)(e * 4503599627370496.0);
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) wsum[warp] = sum;
+  for (int o = 16; o > 0; o >>= 1) fixed += __shfl_xor_sync(0xffffffffu, fixed, o);
+  if (lane == 0) {
+    wsum[warp] = sum;
+    wfixed[warp] = fixed;
+  }
   uint2* out = cand + slot * n;
   for (int i = tid; i < c; i += BS_THREADS) {
     const u64 mine = buf[i];
@@ -345,9 +352,13 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, int V, const fl
   __syncthreads();
   if (warp == 0) {
     sum = lane < BS_THREADS / 32 ? wsum[lane] : 0.0;
+    fixed = lane < BS_THREADS / 32 ? wfixed[lane] : 0;
 #pragma unroll
-    for (int o = BS_THREADS / 64; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) part[slot] = {sum, M, c < n ? c : n};
+    for (int o = BS_THREADS / 64; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      fixed += __shfl_xor_sync(0xffffffffu, fixed, o);
+    }
+    if (lane == 0) part[slot] = {sum + (double)fixed * 2.220446049250313e-16, M, c < n ? c : n};
   }
 }
 
