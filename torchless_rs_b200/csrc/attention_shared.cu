@@ -23,7 +23,7 @@
 //
 // What bounds this is the memory: a tile of head size 128 is 64 KB and takes an SM 1.5 us at the copy rate; the softmax of 16 columns
 // takes a third of that, of 64 columns 1.1 us.  Measured (L2 cold): 4 prompts of 6000 to 16000 tokens x 8 beams, 48 over 8 heads of 128, 206 MB:
-// 47 us, 1.55 us a tile between a start of 5 us (the line, the lists of pages, the first pages) and an end of 5 (a unit's results 2, the
+// 46 us, 1.55 us a tile between a start of 5 us (the line, the lists of pages, the first pages) and an end of 5 (a unit's results 2, the
 // merge 3); 8 prompts of 300 to 4000 tokens x 4, 32 over 8 heads, 84 MB: 24 us; one prompt of 2000 x 4: 10 us, all of it start and
 // end; heads of 64, 6 prompts x 16 beams: 18 us, its tiles 32 KB with a softmax of 64 columns.  Sixteen warps of softmax for 64 columns
 // instead of eight: 2 us more (registers).

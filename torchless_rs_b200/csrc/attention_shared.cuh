@@ -72,7 +72,8 @@ __device__ __forceinline__ int sh_tiles(int common, int own, int beams) { return
 // One warp: the groups' places in the line.  Every unit begins with `totals[2]` places without a tile: that is what beginning a unit and
 // writing one out takes a block, in tiles, so that equal stretches take equal time (4 prompts x 8 beams of the 22B
 // sizes: 57.8 us without them, 55.8 with 2, 53.6 with 4, 52.5 with 6; 8 x 4 of the 7B sizes 27.4, 26.5, 26.9,
-// 27.2).  Where a stretch is a few tiles long there are fewer: more, shorter stretches are then faster.  totals[0], [1]: places in the line, tiles of the longest unit.
+// 27.2).  Where a stretch is a few tiles long there are fewer: more, shorter stretches are then faster.  totals[0], [1]: places in the
+// line, tiles of the longest unit.
 template <int TP, typename T>
 __device__ __forceinline__ void sh_make_line(ShGroup* table, int* totals, const ShArgs<T>& a, int blocks, int lane) {
   int tiles = 0, units = 0, longest = 0;
@@ -177,7 +178,8 @@ __device__ __forceinline__ void sh_page(const ShPiece& p, int i, int& owner, int
 // 7B sizes and 2 us more in 32-bit.)
 //
 // AGAIN: a result that is no number is computed again from the keys that the row sees, one page after the other (the first kernel
-// multiplies values that it does not see by zero).  That is slow, and needed only where the cache holds values that are no numbers.
+// multiplies values that it does not see by zero, and gives a sum that is none where a row's weights left their range).  That is slow, a
+// thread per key, and rare.
 template <int HD, bool EXP2, bool AGAIN, typename T>
 __global__ void __launch_bounds__(SH_MERGE_THREADS)
 attn_shared_merge_kernel(const ShArgs<T> a, const T* __restrict__ k_pages, const T* __restrict__ v_pages) {

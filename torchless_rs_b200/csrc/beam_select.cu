@@ -18,7 +18,7 @@
 // without rounding (below).
 //
 // What bounds it: for many rows the reading of the logits, for few the chain of small steps (loads, barriers, 64-bit exp and log).
-// Measured: 64 sequences x 8 beams x 131072 entries, 268 MB: 57 us (4.7 TB/s); 8 x 4 x 32000: 9 us; 1 x 2 x 256: 7 us, 4 of them the
+// Measured: 64 sequences x 8 beams x 131072 entries, 268 MB: 58 us (4.6 TB/s); 8 x 4 x 32000: 9 us; 1 x 2 x 256: 7 us, 4 of them the
 // second kernel.  One kernel, a cluster of blocks per sequence, took 0 to 1 us more for few rows and 4 to 5 more for 512 (a cluster
 // waits for its slowest block).
 //
