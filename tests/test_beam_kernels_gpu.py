@@ -153,6 +153,33 @@ def test_select_entries_in_an_order(V, n, order):
     _check_select(logits, scores, n)
 
 
+@pytest.mark.parametrize("V,n", [(40, 4), (5000, 2), (5001, 12), (40000, 16), (140001, 8), (9000, 100)])
+@pytest.mark.parametrize("where", ["everywhere", "first tile", "later tile", "spread", "spread, and NaN", "rising, then infinite"])
+def test_select_more_infinite_entries_than_are_asked_for(V, n, where):
+    """Each counts as the largest finite number: the first `n` of a row come with the beam's own score, finite ones beside them do not;
+    other beams of the sequence are as ever."""
+    rng = np.random.default_rng(V + n)
+    x, scores = _rand(rng, 3, 3, V)
+    scores[0] = (-5.0, -30.0, -30.0)          # the infinite ones first
+    scores[1] = (-5.0, -4.0, -6.0)            # and among the others' (these lie some nats below their beam's score)
+    scores[2] = (-90.0, -5.0, -math.inf)      # and last
+    for r in (0, 3, 4, 6):
+        if where == "everywhere":
+            x[r] = np.inf
+        elif where == "first tile":
+            x[r, 2:min(V, 2 + n + 1 + r)] = np.inf
+        elif where == "later tile":
+            x[r, -(n + 1 + r):] = np.inf
+        elif where == "rising, then infinite":
+            x[r].sort()
+            x[r, V // 3::7] = np.inf
+        else:
+            x[r, rng.permutation(V)[:min(V, 3 * n + r)]] = np.inf
+            if "NaN" in where:
+                x[r, rng.permutation(V)[:V // 3]] = np.nan
+    _check_select(x, scores, min(n, V))
+
+
 def test_select_peaked_rows_and_near_ties():
     """One entry holds nearly all weight, and candidates of other beams come within 1e-6 of each other."""
     rng = np.random.default_rng(5)

@@ -181,7 +181,8 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, int V, const fl
 #pragma unroll
         for (int e = k; e < k + 8; ++e) {
           if (v[e] >= bv && v[e] > -INFINITY) {
-            const u64 w = word(fminf(v[e], FLT_MAX), index(i0, e));
+            v[e] = fminf(v[e], FLT_MAX);     // (+inf comes here under every bound; one behind the bound's place is summed as what it counts as)
+            const u64 w = word(v[e], index(i0, e));
             if (w >= b) {
               const int at = atomicAdd(&count, 1);
               if (at < BS_CAP) buf[at] = w;
