@@ -201,6 +201,59 @@ def test_a_first_key_that_stands_out_in_pages_of_another_row(dtype, nh, nkv, hd,
     assert ((got[1:].double() - want.view(4, nh, hd)[1:]).abs() <= bound).all()
 
 
+def _check_far(s):
+    """The bound of `Setting.check` for scores of some dozen: in bfloat16 too a score is a sum of head size products, each step
+    rounded by at most 2^-24 of the largest |score| S, and scaled, so weights are off by a factor of at most exp((head size + 2) 2^-24 S) either
+    way, in the weighted sum and in the sum."""
+    got = s.run()
+    want, mass = s.plain()
+    scores = 2 * (s.hd + 2) * 2.0 ** -24 * s.largest
+    if s.dtype == torch.bfloat16:
+        bound = mass * (2.0 ** -8 + 2.0 ** -12 + scores) + want.abs() * 2.0 ** -8 + 1e-30
+    else:
+        bound = mass * max(2.0 ** -13, scores) + 1e-30
+    assert torch.isfinite(got).all()
+    over = ((got.double() - want).abs() / bound).max().item()
+    assert over <= 1.0, over
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("blocks", [148])
+def test_weights_that_stay_in_range_while_their_sum_does_not(dtype, nh, nkv, hd, blocks, monkeypatch):
+    """The first key that a block sees lies 78 to 90 below the others: from 2^127 / n on the sum of n weights overflows, a signed sum of
+    weighted values need not."""
+    from torchless_rs_b200.csrc import attention_shared
+    monkeypatch.setattr(attention_shared, "_sm_count", lambda device: blocks)
+    for seed, n, c in ((6, 150, 0), (7, 150, 2), (8, 260, 4)):
+        s = Setting(dtype, nh, nkv, hd, [4], [n], [c], seed=seed)
+        s.q.view(-1, nh, hd)[:, :, 0] = 1.0
+        s.k[:, :, :, 0] = 0.0
+        for half in range(156, 181):
+            s.k[s.table[0][0], :, 0, 0] = -0.5 * half / s.scale
+            _check_far(s)
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("blocks", [148])
+@pytest.mark.parametrize("count", [64, 128, 256, 1000])
+def test_many_keys_of_one_height_far_above_the_first(dtype, nh, nkv, hd, blocks, count, monkeypatch):
+    """`count` keys 80 to 89 above those before them, with values of 0.1 and less: the sum of weights leaves its range before the weighted sum
+    does, in one piece or where pieces are joined."""
+    from torchless_rs_b200.csrc import attention_shared
+    monkeypatch.setattr(attention_shared, "_sm_count", lambda device: blocks)
+    for first in (1, 64, 200):
+        n = first + count
+        s = Setting(dtype, nh, nkv, hd, [3], [n], [(n - 1) // PAGE], seed=first, spread=0.3)
+        s.v.mul_(0.05)
+        s.q.view(-1, nh, hd)[:, :, 0] = 1.0
+        s.k[:, :, :, 0] = 0.0
+        place = torch.arange(first, n, device=DEV)
+        page = torch.tensor(s.table, device=DEV)[:, place // PAGE]           # [rows, keys]
+        for half in range(160, 179):
+            s.k[page, :, place % PAGE, 0] = 0.5 * half / s.scale
+            _check_far(s)
+
+
 @pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
 def test_scores_far_apart_and_scale(dtype, nh, nkv, hd):
     s = Setting(dtype, nh, nkv, hd, [4, 2], [700, 90], [9, 1], spread=0.2, seed=1)

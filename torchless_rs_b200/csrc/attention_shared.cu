@@ -46,8 +46,8 @@
 #define SH_STRIDE (HEAD_DIM + 2)                    // floats of a partial result: weighted sum, maximum, sum
 #define SH_MAX_HEADS 16                             // query heads per key/value head
 // A column's reference moves two tiles after a score has exceeded it by 2^60 (in between weights reach what the two tiles' scores exceed it
-// by; at 2^127 the result is none and is computed again), so that no tile waits for a maximum; rounding to bfloat16 is relative.  A sum of
-// weights below 2^-60 is not taken either: what is lost below 2^-126 is then no more than 2^-66 of it.
+// by; where one weight or their sum comes to 2^128 the result is none and is computed again), so that no tile waits for a maximum; rounding to
+// bfloat16 is relative.  A sum of weights below 2^-60 is not taken either: what is lost below 2^-126 is then no more than 2^-66 of it.
 #define SH_SLACK 60.0f
 #define SH_LEAST 8.67361737988403547e-19f            // 2^-60
 
@@ -551,7 +551,7 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           const int from = 2 * p.tile - p.common, to = min(2 * last, p.pages) - 1 - p.common;
           const bool any = from < 0 || (my_beam >= from / p.own && my_beam <= to / p.own);
           dst[0] = any ? ref_s[my_col] : -INFINITY;
-          dst[1] = any && !(sum >= SH_LEAST) ? NAN : sum;       // (too little of it is left)
+          dst[1] = any && !(sum >= SH_LEAST && sum < INFINITY) ? NAN : sum;     // (too little of it is left, or it overflowed)
         }
         sh_park(&pv_done[(n - 1) & 1], (uint32_t)((n - 1) >> 1) & 1u, abort_flag, 13);
         tc_fence_after();

@@ -252,7 +252,7 @@ attn_shared_merge_kernel(const ShArgs<T> a, const T* __restrict__ k_pages, const
   }
   store(l);
   if constexpr (AGAIN) {
-    bool bad = false;
+    bool bad = !isfinite(l);       // (a sum that overflowed would make zeros of a weighted sum that did not)
 #pragma unroll
     for (int e = 0; e < E; ++e) bad |= !isfinite(acc[e] / l);
     if (!__any_sync(0xffffffffu, bad)) return;
