@@ -218,7 +218,7 @@ def _check_far(s):
 
 
 @pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
-@pytest.mark.parametrize("blocks", [148])
+@pytest.mark.parametrize("blocks", [1, 148])
 def test_weights_that_stay_in_range_while_their_sum_does_not(dtype, nh, nkv, hd, blocks, monkeypatch):
     """The first key that a block sees lies 78 to 90 below the others: from 2^127 / n on the sum of n weights overflows, a signed sum of
     weighted values need not."""
@@ -234,7 +234,7 @@ def test_weights_that_stay_in_range_while_their_sum_does_not(dtype, nh, nkv, hd,
 
 
 @pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
-@pytest.mark.parametrize("blocks", [148])
+@pytest.mark.parametrize("blocks", [1, 2, 148])
 @pytest.mark.parametrize("count", [64, 128, 256, 1000])
 def test_many_keys_of_one_height_far_above_the_first(dtype, nh, nkv, hd, blocks, count, monkeypatch):
     """`count` keys 80 to 89 above those before them, with values of 0.1 and less: the sum of weights leaves its range before the weighted sum

@@ -173,7 +173,7 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   float* red_s = (float*)(table + SH_MAX_GROUPS);      // [4][N]
   float* ref_s = red_s + 4 * N;                        // [N]
   float* neg_s = ref_s + N;                            // [N]: the negated references
-  float* al_s = neg_s + N;                             // [N]
+  float* al_s = neg_s + N;                             // [N]: square roots of the factors by which what is summed so far shrinks
   uint64_t* k_full = (uint64_t*)(al_s + N);
   uint64_t* k_empty = k_full + Z::KS;
   uint64_t* v_full = k_empty + Z::KS;
@@ -483,12 +483,15 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
               const float now = m > old + SH_SLACK ? m : old;
               ref_s[first_col + key] = now;
               neg_s[first_col + key] = -now;
-              al_s[first_col + key] = now == old ? 1.0f : sh_ex2(old - now);
+              // (the root of the factor, which is taken twice: the sums so far may have come to 2^128 against the old reference and
+              // weigh something below it, where the factor itself, from 2^-127 on, would be flushed to zero)
+              al_s[first_col + key] = now == old ? 1.0f : sh_ex2(0.5f * (old - now));
             }
             meet();
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-              l[c] *= al_s[first_col + c];
+              const float root = al_s[first_col + c];
+              l[c] = l[c] * root * root;
               s[c] += neg[c];
             }
             if (j > p.tile) {
@@ -498,7 +501,10 @@ FN(attn_shared_kernel)(const __grid_constant__ CUtensorMap tm_k, const __grid_co
               float o[NC];
               sh_tmem_ld<NC>(tmem_o + t_lane + first_col, o);
 #pragma unroll
-              for (int c = 0; c < NC; ++c) o[c] *= al_s[first_col + c];
+              for (int c = 0; c < NC; ++c) {
+                const float root = al_s[first_col + c];
+                o[c] = o[c] * root * root;
+              }
 #pragma unroll
               for (int c = 0; c < NC; c += 8) sh_tmem_st8(tmem_o + t_lane + first_col + c, o + c);
               sh_tmem_st_wait();
