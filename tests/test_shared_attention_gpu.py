@@ -254,6 +254,25 @@ def test_many_keys_of_one_height_far_above_the_first(dtype, nh, nkv, hd, blocks,
             _check_far(s)
 
 
+@pytest.mark.parametrize("dtype,nh,nkv,hd", [(torch.bfloat16, 1, 1, 64), (torch.bfloat16, 1, 1, 128), (torch.float32, 1, 1, 128)])
+@pytest.mark.parametrize("high", [100.0, 111.0, 120.0])
+def test_pieces_whose_references_say_little_of_their_weights(dtype, nh, nkv, hd, high, monkeypatch):
+    """Two blocks.  The first has the common keys, 81 above the first of them; the second begins with a key of row 0's own, `high` above all
+    that, and row 1's own keys lie 38 below that one: most of what row 1 sees is in the first block, whose reference is the lower by far."""
+    from torchless_rs_b200.csrc import attention_shared
+    monkeypatch.setattr(attention_shared, "_sm_count", lambda device: 2)
+    monkeypatch.setattr(attention_shared, "PER_SM", {torch.bfloat16: 1, torch.float32: 1})
+    s = Setting(dtype, nh, nkv, hd, [2], [8 * PAGE], [4], seed=12, spread=0.3)
+    s.q.view(-1, nh, hd)[:, :, 0] = 1.0
+    s.k[:, :, :, 0] = 0.0
+    common, own0, own1 = s.table[0][:4], s.table[0][4:8], s.table[1][4:8]
+    s.k[common, :, :, 0] = 81.0 / s.scale
+    s.k[common[0], :, 0, 0] = 0.0
+    s.k[own0, :, :, 0] = high / s.scale
+    s.k[own1, :, :, 0] = (high - 38.0) / s.scale
+    _check_far(s)
+
+
 @pytest.mark.parametrize("dtype,nh,nkv,hd", HEADS)
 def test_scores_far_apart_and_scale(dtype, nh, nkv, hd):
     s = Setting(dtype, nh, nkv, hd, [4, 2], [700, 90], [9, 1], spread=0.2, seed=1)

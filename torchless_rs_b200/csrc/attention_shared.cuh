@@ -226,7 +226,10 @@ attn_shared_merge_kernel(const ShArgs<T> a, const T* __restrict__ k_pages, const
   for (int s0 = 0; s0 < parts; s0 += 32) {
     // references and sums of 32 pieces (a piece in which this row sees no key has a reference of -inf)
     const float2 rs = s0 + lane < parts ? *reinterpret_cast<const float2*>(src + (s0 + lane) * STRIDE + HD) : make_float2(-INFINITY, 0.0f);
-    float top = fmaxf(m, rs.x);
+    // What a piece weighs is its sum against its reference.  Where the reference is not the maximum, the sum (2^-60 to 2^128) says
+    // as much as the reference, and its power of two counts with it: a piece's factor then is 2^-127 at the least where the piece
+    // matters, which 32 bits hold (not flushed) to 2^-22.
+    float top = fmaxf(m, EXP2 && rs.x > -INFINITY ? rs.x + (float)((int)(__float_as_uint(rs.y) >> 23 & 255u) - 127) : rs.x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     auto weight = [&](float ref) { return ref == -INFINITY ? 0.0f : EXP2 ? exp2f(ref - top) : expf(ref - top); };
