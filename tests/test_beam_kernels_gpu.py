@@ -180,6 +180,17 @@ def test_select_more_infinite_entries_than_are_asked_for(V, n, where):
     _check_select(x, scores, min(n, V))
 
 
+@pytest.mark.parametrize("V,n", [(300, 8), (5000, 16), (20001, 24), (70000, 100)])
+def test_select_zeros_of_either_sign_are_equal(V, n):
+    rng = np.random.default_rng(V)
+    x = np.where(rng.random((6, V)) < 0.5, np.float32(0.0), np.float32(-0.0))
+    x[rng.random(x.shape) < 0.3] = -1.0
+    x[0, :V // 2] = np.float32(-0.0)
+    x[0, V // 2:] = np.float32(0.0)
+    x[4] = np.float32(-0.0)
+    _check_select(x, np.full((2, 3), -1.5, dtype=np.float32), n)
+
+
 def test_select_peaked_rows_and_near_ties():
     """One entry holds nearly all weight, and candidates of other beams come within 1e-6 of each other."""
     rng = np.random.default_rng(5)

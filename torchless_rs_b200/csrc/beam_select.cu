@@ -137,8 +137,8 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, int V, const fl
       for (int j = 0; j < 16; ++j) x[j] = fmaxf(x[j], -INFINITY);
     }
   };
-  // A word orders entries by value, equal ones by index, lowest first.
-  auto word = [&](float x, int i) { return ((u64)bs_key(x) << 32) | (uint32_t)~i; };
+  // A word orders entries by value, equal ones (zeros of either sign among them) by index, lowest first.
+  auto word = [&](float x, int i) { return ((u64)bs_key(x + 0.0f) << 32) | (uint32_t)~i; };
 
   float x[16];
   load(first, x);
