@@ -191,6 +191,22 @@ def test_select_zeros_of_either_sign_are_equal(V, n):
     _check_select(x, np.full((2, 3), -1.5, dtype=np.float32), n)
 
 
+@pytest.mark.parametrize("V", [999, 4099, 9001, 9002, 9004, 50257, 70003])
+@pytest.mark.parametrize("layout", ["contiguous", "a view of wider rows", "a view whose rows begin alike"])
+def test_select_beams_that_are_alike(V, layout):
+    """Beams of one sequence with the same logits and the same score: every token comes from the lower beam first, then from the other,
+    wherever in memory their rows begin."""
+    rng = np.random.default_rng(V)
+    wide = {"contiguous": V, "a view of wider rows": V + 5, "a view whose rows begin alike": (V + 7) // 4 * 4}[layout]
+    store = torch.from_numpy(rng.standard_normal((10, wide)).astype(np.float32) * np.float32(0.5)).cuda()
+    x = store[:, wide - V:]
+    x[1:4] = x[0].clone()                     # sequence 0: beams 0 to 3
+    x[7], x[8] = x[5].clone(), x[5].clone()   # sequence 1: beams 0, 2 and 3
+    scores = np.full((2, 5), -3.25, dtype=np.float32)
+    for n in (8, 30, 100):
+        _check_select(x, scores, n)
+
+
 def test_select_peaked_rows_and_near_ties():
     """One entry holds nearly all weight, and candidates of other beams come within 1e-6 of each other."""
     rng = np.random.default_rng(5)

@@ -92,7 +92,13 @@ struct BsPart {
 #define BS_PER_SM 4                // resident blocks
 
 // GS threads form a group (256 / GS >= 2 n groups, or as many as there are threads).
-template <int GS>
+//
+// ALIKE: all rows begin at the same place between two 16-byte boundaries of memory (their distance is a multiple of 16 bytes, or there is
+// one): entries are read in fours on those boundaries.  Otherwise they are read one by one, a row's first by the first thread.  Either way
+// an entry's place in its row alone says which thread adds it, and when, so rows with the same entries have the same sum to the last bit, and
+// beams that are alike tie.  (Fours on the boundaries of every row instead: 64 x 8 x 131071 entries 66 us against 61.5, 64 x 8 x 50257 34.7 against
+// 35.5, 64 x 4 x 32003 18.0 against 18.5.)
+template <int GS, bool ALIKE>
 __global__ void __launch_bounds__(BS_THREADS, BS_PER_SM)
 beam_rows_kernel(const float* __restrict__ logits, long long ld, int V, const float* __restrict__ scores, int n, int chunk,
                  BsPart* __restrict__ part, uint2* __restrict__ cand) {
@@ -109,21 +115,26 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, int V, const fl
   const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t slot = (size_t)row * gridDim.x + blockIdx.x;
   const float score = scores[row];
-  // The entries in fours on 16-byte boundaries of memory: `shift` entries before the row's first belong to the row before.
+  // In fours: `shift` entries before the row's first belong to the row before.
   const float* x0 = logits + (size_t)row * ld;
-  const int shift = (int)(((uintptr_t)x0 >> 2) & 3);
+  const int shift = ALIKE ? (int)(((uintptr_t)x0 >> 2) & 3) : 0;
   const int first = blockIdx.x * chunk - shift, end = min(first + chunk, V);
   // Entry j of this thread in the tile that begins at i0.
-  auto index = [&](int i0, int j) { return i0 + ((j >> 2) * BS_THREADS + tid) * 4 + (j & 3); };
-  const float* mine0 = x0 + first + tid * 4;
+  auto index = [&](int i0, int j) { return ALIKE ? i0 + ((j >> 2) * BS_THREADS + tid) * 4 + (j & 3) : i0 + j * BS_THREADS + tid; };
+  const float* mine0 = x0 + first + (ALIKE ? tid * 4 : tid);
   bool nans = false;              // entries that are NaN were met: they become -inf as they are loaded
   auto load = [&](int i0, float (&x)[16]) {
     if (i0 >= 0 && i0 + BS_TILE <= end) {              // (a whole tile)
       const float* p = mine0 + (i0 - first);
+      if constexpr (ALIKE) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float4 v = __ldcs(reinterpret_cast<const float4*>(p + k * BS_THREADS * 4));
-        x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
+        for (int k = 0; k < 4; ++k) {
+          const float4 v = __ldcs(reinterpret_cast<const float4*>(p + k * BS_THREADS * 4));
+          x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = __ldcs(p + j * BS_THREADS);
       }
     } else {
 #pragma unroll
@@ -550,8 +561,8 @@ extern "C" long long tl_beam_scratch_bytes(int rows, int V, int n) {
 template <int GS>
 static int bs_run(const float* logits, long long ld, int S, int B, int V, const float* scores, int n, void* scratch, float* values,
                   int* beams, int* tokens, cudaStream_t stream) {
-  const bool shifted = ld % 4 != 0 || ((uintptr_t)logits & 15);
   const int rows = S * B;
+  const bool alike = rows == 1 || ld % 4 == 0, shifted = alike && ((uintptr_t)logits & 15);
   int chunk = bs_chunk(rows, V);
   // Longer parts where they leave no more candidates than the second kernel's threads hold: one sequence of 8 beams, 16 continuations, 262144
   // entries: parts of one tile 33 us, of 8 tiles 19 us; 16 beams, 32 continuations, 131072 entries 146 and 33.  (More than 8
@@ -560,7 +571,8 @@ static int bs_run(const float* logits, long long ld, int S, int B, int V, const 
   const int parts = bs_parts(V, chunk, shifted);
   BsPart* part = (BsPart*)scratch;
   uint2* cand = (uint2*)(part + (size_t)rows * parts);
-  const int st = tl_launch(beam_rows_kernel<GS>, dim3(parts, rows), dim3(BS_THREADS), 0, stream, logits, ld, V, scores, n, chunk, part, cand);
+  const int st = alike ? tl_launch(beam_rows_kernel<GS, true>, dim3(parts, rows), dim3(BS_THREADS), 0, stream, logits, ld, V, scores, n, chunk, part, cand)
+                       : tl_launch(beam_rows_kernel<GS, false>, dim3(parts, rows), dim3(BS_THREADS), 0, stream, logits, ld, V, scores, n, chunk, part, cand);
   if (st) return st;
   const long long total = (long long)B * parts * n;
   auto merge = [&](auto kernel) {
