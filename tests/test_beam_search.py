@@ -373,3 +373,41 @@ def test_step_arrays_are_laid_out_as_before_and_groups_behind_them():
                                                              "want_rows", "token_from"}
     g = RowGroups([4, 1], [200, 7], [3, 0])
     assert g.key() == ((4, 1), 256, 1) and g.key() == RowGroups([4, 1], [190, 7], [2, 0]).key()
+
+
+@pytest.mark.parametrize("requests", [None, [PagedLatentRequest(24)], [PagedKVRequest(2, 16, window=100), PagedKVRequest(2, 16)]])
+@pytest.mark.parametrize("have,wanted", [(0, 1), (64, 65), (64, 300), (70, 129), (70, 71), (128, 193)])
+def test_a_fork_after_a_step_that_did_not_run_to_its_end(requests, have, wanted):
+    """The table has grown and the length has not: the pages beyond the length stay the source's own."""
+    c = _cache(requests)
+    a, b, d = c.acquire(3)
+    if have:
+        _write(c, [a], [have], [1])
+    c.prepare([a], [wanted])             # (and the step raises)
+    c.check()
+    c.fork([a, a], [b, d])
+    c.check()
+    assert all(g.n_cols[s] == -(-have // PAGE) for g in c.paged for s in (b, d))
+    for s, t in ((a, 1), (b, 2), (d, 3)):
+        _write(c, [s], [wanted], [t])
+    for s, t in ((a, 1), (b, 2), (d, 3)):
+        _expect(c, s, [(1, 0, have), (t, have, wanted)])
+    c.prepare([a, b], [wanted + 100] * 2)
+    new = c.reorder([a, b, d], [0, 0, 1])
+    _write(c, new, [wanted + 70] * 3, [5, 6, 7])
+    for s, t, o in zip(new, (5, 6, 7), (1, 1, 2)):
+        _expect(c, s, [(1, 0, have), (o, have, wanted), (t, wanted, wanted + 70)])
+    c.release([a, b, d])
+    c.check()
+    assert all(g.pool.held_count == 0 and not g.holders.any() for g in c.paged)
+
+
+def test_the_check_refuses_a_shared_page_beyond_a_length():
+    c = _cache([PagedKVRequest(2, 16)])
+    a, b = c.acquire(2)
+    _write(c, [a], [128], [1])
+    c.fork([a], [b])
+    c.check()
+    c.lengths[b] = 64
+    with pytest.raises(CacheStateError, match="beyond"):
+        c.check()

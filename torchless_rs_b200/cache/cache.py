@@ -119,18 +119,22 @@ class PagedGroup:
         self.holders[pages] -= 1
         self.pool.give_back(p for p in pages if self.holders[p] == 0)
 
-    def fork(self, src: Sequence[int], dst: Sequence[int]) -> None:
-        """Each slot dst[i] lets go of what it holds and holds the pages of src[i] from now on."""
+    def fork(self, src: Sequence[int], dst: Sequence[int], lengths: Sequence[int]) -> None:
+        """Each slot dst[i] lets go of what it holds and holds the pages of the first lengths[i] positions of src[i] from now on.  (A
+        step that was prepared and did not run to its end has left src[i] further pages, which it will write to: those stay its own.)"""
         cols = max(self.n_cols[s] for s in dst)
         gone = self.table_host[dst, :cols].ravel()
         gone = gone[gone >= 0]
         np.subtract.at(self.holders, gone, 1)
-        held = self.table_host[src, :max(self.n_cols[s] for s in src)]
-        self.table_host[dst] = self.table_host[src]
+        keep = [min(self.n_cols[a], pages_for(n)) for a, n in zip(src, lengths)]
+        rows = self.table_host[src]
+        held = rows[:, :max(self.n_cols[a] for a in src)]
+        held[np.arange(held.shape[1]) >= np.asarray(keep)[:, None]] = -1
+        self.table_host[dst] = rows
         np.add.at(self.holders, held[held >= 0], 1)
         self.pool.give_back(np.unique(gone[self.holders[gone] == 0]).tolist())
-        for a, b in zip(src, dst):
-            self.first_live[b], self.n_cols[b] = self.first_live[a], self.n_cols[a]
+        for a, b, c in zip(src, dst, keep):
+            self.first_live[b], self.n_cols[b] = self.first_live[a], c
         self._dirty.update(dst)
 
     def writes_into_shared(self, slots: Sequence[int], lengths: Sequence[int]) -> List[int]:
@@ -444,7 +448,7 @@ class Cache:
         if not src:
             return
         for g in self.paged:
-            g.fork(src, dst)
+            g.fork(src, dst, [self.lengths[a] for a in src])
             g.upload()
         for g in self.states:
             g.fork(src, dst, self.dtype)
@@ -543,6 +547,8 @@ class Cache:
                     raise CacheStateError(f"free slot {s} still holds pages")
                 if len(set(pages)) != len(pages):
                     raise CacheStateError(f"slot {s} holds a page twice")
+                if any(p >= 0 and g.holders[p] > 1 for p in g.table_host[s, pages_for(self.lengths[s]):]):
+                    raise CacheStateError(f"slot {s} holds a page beyond its length that others hold too")
                 for p in pages:
                     if not g.pool.is_held(p):
                         raise CacheStateError(f"page {p} is in a table but free")
