@@ -411,3 +411,45 @@ def test_the_check_refuses_a_shared_page_beyond_a_length():
     c.lengths[b] = 64
     with pytest.raises(CacheStateError, match="beyond"):
         c.check()
+
+
+def _state(c):
+    return [(g.table_host.copy(), g.table_dev.clone(), g.holders.copy(), list(g.n_cols), list(g.first_live), g.pool.free_count) for g in c.paged], \
+        [g.storage.clone() for g in c.states], list(c.lengths)
+
+
+def _same(before, c):
+    paged, states, lengths = _state(c)
+    for x, y in zip(before[0], paged):
+        assert all(np.array_equal(np.asarray(u), np.asarray(v)) for u, v in zip(x, y))
+    return all(torch.equal(x, y) for x, y in zip(before[1], states)) and before[2] == lengths
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_copies_that_are_refused_change_nothing(which, monkeypatch):
+    """As where another device is the current one: the copies raise before anything is launched."""
+    c = _cache([PagedKVRequest(2, 16), PagedKVRequest(2, 16, window=100), StateRequest((3, 2))])
+    a, b, d = c.acquire(3)
+    _write(c, [a], [90], [1])
+    _write(c, [d], [40], [2])
+    before = _state(c)
+
+    def refuse(*args):
+        raise RuntimeError("not on this device")
+    monkeypatch.setattr(c.states[0], "fork", refuse)
+    with pytest.raises(RuntimeError, match="not on this device"):
+        c.fork([a, a], [b, d])
+    c.check()
+    assert _same(before, c)
+    monkeypatch.undo()
+    c.fork([a, a], [b, d])
+    before = _state(c)
+    monkeypatch.setattr(c.paged[which], "copy_pages", refuse)
+    with pytest.raises(RuntimeError, match="not on this device"):
+        c.prepare([a, b, d], [91, 150, 300])
+    c.check()
+    assert _same(before, c)
+    monkeypatch.undo()
+    _write(c, [a, b, d], [91, 150, 300], [1, 2, 3])
+    for s, t, n in ((a, 1, 91), (b, 2, 150), (d, 3, 300)):
+        _expect(c, s, [(1, 0, 90), (t, 90, n)])

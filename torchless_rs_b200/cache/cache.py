@@ -151,19 +151,25 @@ class PagedGroup:
                 left[page] = holders - 1
         return out
 
-    def unshare(self, slots: Sequence[int], lengths: Sequence[int]) -> None:
-        """Gives each of `slots` a page of its own in the place of the page of position lengths[i], with the positions before it."""
+    def begun_copies(self, slots: Sequence[int], lengths: Sequence[int]) -> List[int]:
+        """A new page for each of `slots` with what its page of position lengths[i] holds before that; no table names it yet."""
         if not slots:
-            return
-        cols = [n // PAGE for n in lengths]
-        src = [int(self.table_host[s, c]) for s, c in zip(slots, cols)]
-        dst = self.pool.take(len(slots))
-        for s, c, old, new in zip(slots, cols, src, dst):
-            self.holders[old] -= 1
+            return []
+        new = self.pool.take(len(slots))
+        try:
+            self.copy_pages([int(self.table_host[s, n // PAGE]) for s, n in zip(slots, lengths)], new, [n % PAGE for n in lengths])
+        except Exception:
+            self.pool.give_back(new)
+            raise
+        return new
+
+    def unshare(self, slots: Sequence[int], lengths: Sequence[int], pages: Sequence[int]) -> None:
+        """Puts the pages of `begun_copies` in the place of the pages of position lengths[i]."""
+        for s, n, new in zip(slots, lengths, pages):
+            self.holders[self.table_host[s, n // PAGE]] -= 1
             self.holders[new] = 1
-            self.table_host[s, c] = new
+            self.table_host[s, n // PAGE] = new
             self._dirty.add(s)
-        self.copy_pages(src, dst, [n % PAGE for n in lengths])
 
     def copy_pages(self, src: Sequence[int], dst: Sequence[int], counts: Sequence[int]) -> None:
         """The first counts[i] positions of page src[i] into page dst[i], in all layers."""
@@ -447,11 +453,11 @@ class Cache:
             raise CacheStateError("a sequence slot is written twice, or both copied from and written")
         if not src:
             return
+        for g in self.states:            # (before the tables: a copy may be refused, where another device is the current one)
+            g.fork(src, dst, self.dtype)
         for g in self.paged:
             g.fork(src, dst, [self.lengths[a] for a in src])
             g.upload()
-        for g in self.states:
-            g.fork(src, dst, self.dtype)
         for a, b in zip(src, dst):
             self.lengths[b] = self.lengths[a]
 
@@ -488,7 +494,7 @@ class Cache:
     def prepare(self, slots: Sequence[int], new_lens: Sequence[int]) -> None:
         """Makes room for each sequence to reach its new length, gives a sequence that would write to a page
         which others hold too a page of its own, and brings the device's page tables up to date.  Nothing
-        changes if there is no room."""
+        changes if there is no room or a copy is refused."""
         for s in slots:
             if not self.slots.is_held(s):
                 raise CacheStateError(f"sequence slot {s} is used but is not held")
@@ -507,8 +513,18 @@ class Cache:
                 raise CacheCapacityError(
                     f"the cache is full: this step needs {need} more pages of {PAGE} tokens, "
                     f"{g.pool.free_count} of {g.n_pages} are free")
-        for g, shared in zip(self.paged, copies):
-            g.unshare([slots[i] for i in shared], [past[i] for i in shared])
+        # The copies come before the tables change: they may be refused (where another device is the current one).
+        copies = [([slots[i] for i in shared], [past[i] for i in shared]) for shared in copies]
+        pages: List[List[int]] = []
+        try:
+            for g, (of, lens) in zip(self.paged, copies):
+                pages.append(g.begun_copies(of, lens))
+        except Exception:
+            for g, got in zip(self.paged, pages):
+                g.pool.give_back(got)
+            raise
+        for g, (of, lens), got in zip(self.paged, copies, pages):
+            g.unshare(of, lens, got)
             for s, n in zip(slots, new_lens):
                 g.grow(s, n)
             g.upload()
