@@ -453,3 +453,26 @@ def test_copies_that_are_refused_change_nothing(which, monkeypatch):
     _write(c, [a, b, d], [91, 150, 300], [1, 2, 3])
     for s, t, n in ((a, 1, 91), (b, 2, 150), (d, 3, 300)):
         _expect(c, s, [(1, 0, 90), (t, 90, n)])
+
+
+def test_steps_of_sequences_that_were_never_forked_look_for_no_shared_pages(monkeypatch):
+    """A step's host time for them is what it was: the pages' holders are looked at from a fork on, until the cache is empty."""
+    c = _cache()
+    looked = []
+    for g in c.paged:
+        monkeypatch.setattr(g, "writes_into_shared", lambda *a, of=type(g).writes_into_shared, g=g: looked.append(1) or of(g, *a))
+    a, b = c.acquire(2)
+    _write(c, [a, b], [70, 3], [1, 2])
+    _write(c, [a, b], [71, 4], [1, 2])
+    assert not looked
+    c.fork([a], [b])
+    _write(c, [a, b], [72, 72], [1, 2])
+    assert looked
+    c.release([a])
+    _write(c, [b], [73], [2])
+    assert len(looked) == 2 * len(c.paged)
+    c.release([b])
+    (a,) = c.acquire(1)
+    _write(c, [a], [70], [1])
+    _write(c, [a], [71], [1])
+    assert len(looked) == 2 * len(c.paged)

@@ -74,6 +74,7 @@ class PagedGroup:
         self.n_pages = n_pages
         self.pool = FreeList(n_pages, "cache page")
         self.holders = np.zeros(n_pages, dtype=np.int32)   # sequences that hold a page
+        self.forked = False                 # several may hold one page: a fork has been made since the pool was last empty
         if isinstance(request, PagedLatentRequest):
             shape = (len(self.layers), n_pages, PAGE * request.width)
         else:
@@ -118,6 +119,7 @@ class PagedGroup:
         pages = [int(p) for p in pages if p >= 0]
         self.holders[pages] -= 1
         self.pool.give_back(p for p in pages if self.holders[p] == 0)
+        self.forked = self.forked and self.pool.held_count > 0
 
     def fork(self, src: Sequence[int], dst: Sequence[int], lengths: Sequence[int]) -> None:
         """Each slot dst[i] lets go of what it holds and holds the pages of the first lengths[i] positions of src[i] from now on.  (A
@@ -133,6 +135,7 @@ class PagedGroup:
         self.table_host[dst] = rows
         np.add.at(self.holders, held[held >= 0], 1)
         self.pool.give_back(np.unique(gone[self.holders[gone] == 0]).tolist())
+        self.forked = True
         for a, b, c in zip(src, dst, keep):
             self.first_live[b], self.n_cols[b] = self.first_live[a], c
         self._dirty.update(dst)
@@ -506,7 +509,7 @@ class Cache:
                     f"a sequence of {n} tokens is longer than the cache was sized for "
                     f"({self.max_seq_len})")
         past = [self.lengths[s] for s in slots]
-        copies = [g.writes_into_shared(slots, past) if g.pool.held_count else [] for g in self.paged]
+        copies = [g.writes_into_shared(slots, past) if g.forked else [] for g in self.paged]
         for g, shared in zip(self.paged, copies):
             need = sum(g.pages_needed(s, n) for s, n in zip(slots, new_lens)) + len(shared)
             if need > g.pool.free_count:
@@ -514,7 +517,7 @@ class Cache:
                     f"the cache is full: this step needs {need} more pages of {PAGE} tokens, "
                     f"{g.pool.free_count} of {g.n_pages} are free")
         # The copies come before the tables change: they may be refused (where another device is the current one).
-        copies = [([slots[i] for i in shared], [past[i] for i in shared]) for shared in copies]
+        copies = [([slots[i] for i in shared], [past[i] for i in shared]) if shared else ((), ()) for shared in copies]
         pages: List[List[int]] = []
         try:
             for g, (of, lens) in zip(self.paged, copies):
