@@ -476,3 +476,25 @@ def test_steps_of_sequences_that_were_never_forked_look_for_no_shared_pages(monk
     _write(c, [a], [70], [1])
     _write(c, [a], [71], [1])
     assert len(looked) == 2 * len(c.paged)
+
+
+@pytest.mark.parametrize("lens,max_tokens", [((64, 63), 1), ((128, 127, 126), 1), ((64, 63, 10), 3), ((200, 192, 190, 1), 40)])
+def test_the_command_line_makes_room_for_every_prompt(lens, max_tokens, monkeypatch, tmp_path, capsys):
+    """A prompt that ends inside a page may need more pages than a longer one: the cache holds all prompts' beams at once."""
+    from types import SimpleNamespace
+    from torchless_rs_b200 import api, config
+    prompts, seen = [[7] * n for n in lens], {}
+
+    class FakeModel:
+        def generate_beams(self, prompts, max_tokens, beams, **kw):
+            seen["batches"] = plan_beam_batches([len(p) for p in prompts], max_tokens, beams, seen["max_tokens"], seen["max_batch"])
+            return [SimpleNamespace(tokens=[1]) for _ in prompts]
+
+    def load(where, dtype, max_tokens, max_batch, max_seq_len):
+        seen.update(max_tokens=max_tokens, max_batch=max_batch)
+        return FakeModel()
+    monkeypatch.setattr(config, "load_config", lambda where: SimpleNamespace(max_position_embeddings=4096, bos_token_id=1, eos_token_ids=()))
+    monkeypatch.setattr(api, "load", load)
+    text = " ; ".join(" ".join(str(t) for t in p) for p in prompts)
+    assert cli.main(["--beams", "4", "--max-tokens", str(max_tokens), str(tmp_path), text]) == 0, capsys.readouterr().err
+    assert seen["batches"] == [list(range(len(lens)))]

@@ -206,11 +206,12 @@ def main(argv: Optional[List[str]] = None, prog: str = "torchless") -> int:
               file=sys.stderr)
         return 1
     max_tokens = min(max_tokens, max_seq_len - longest + 1)
-    per_seq = (min(max_seq_len, longest + max_tokens) + 63) // 64 * 64
+    cache_tokens = (min(max_seq_len, longest + max_tokens) + 63) // 64 * 64 * len(prompts)
     rows = len(prompts)
     if opts["beams"]:
         from .engine.beam import held_pages
-        per_seq = held_pages(longest, max_tokens, opts["beams"]) * 64
+        # (each prompt for itself: one that ends inside a page may need more than a longer one that fills its last)
+        cache_tokens = sum(held_pages(len(p), max_tokens, opts["beams"]) for p in prompts) * 64
         rows *= opts["beams"]
     if opts["debug"]:
         print(f"Loading {model_dir} ({opts['dtype']}), {len(prompts)} prompt(s), "
@@ -225,10 +226,10 @@ def main(argv: Optional[List[str]] = None, prog: str = "torchless") -> int:
                 write_random_model(config, model_dir, opts["weights_seed"], api.parse_dtype(opts["dtype"]),
                                    "cuda:0")
             model = api.from_random(config, seed=opts["weights_seed"], dtype=opts["dtype"],
-                                    max_tokens=per_seq * len(prompts), max_batch=rows,
+                                    max_tokens=cache_tokens, max_batch=rows,
                                     max_seq_len=max_seq_len)
         else:
-            model = api.load(model_dir, dtype=opts["dtype"], max_tokens=per_seq * len(prompts),
+            model = api.load(model_dir, dtype=opts["dtype"], max_tokens=cache_tokens,
                              max_batch=rows, max_seq_len=max_seq_len)
     except Exception as e:
         print(f"Error: {e}", file=sys.stderr)
