@@ -498,3 +498,15 @@ def test_the_command_line_makes_room_for_every_prompt(lens, max_tokens, monkeypa
     text = " ; ".join(" ".join(str(t) for t in p) for p in prompts)
     assert cli.main(["--beams", "4", "--max-tokens", str(max_tokens), str(tmp_path), text]) == 0, capsys.readouterr().err
     assert seen["batches"] == [list(range(len(lens)))]
+
+
+@pytest.mark.parametrize("penalty", [400.0, -400.0, 1e300])
+def test_length_penalties_that_leave_the_range_of_numbers_are_refused(penalty):
+    """16^400 is no number, 16^-400 is zero: refused before a sequence is started."""
+    eng = ScriptedEngine(4, 5)
+    with pytest.raises(ValueError, match="penalty"):
+        generate_beams(eng, select, [[1]], 16, 4, penalty, cache_tokens=999, max_batch=4)
+    assert len(eng.free) == 4
+    for fine in (250.0, -250.0):
+        assert generate_beams(eng, select, [[1]], 16, 4, fine, cache_tokens=999, max_batch=4)[0].hypotheses
+    assert generate_beams(eng, select, [[1]], 1, 4, penalty, cache_tokens=999, max_batch=4)[0].hypotheses       # 1 to any power

@@ -145,6 +145,8 @@ def generate_beams(engine, select: Callable, prompts: Sequence[Sequence[int]], m
         raise ValueError(f"n_best must lie in 1 to {beams}, got {n_best}")
     if not math.isfinite(length_penalty):
         raise ValueError("the length penalty must be a finite number")
+    if max_tokens > 1 and abs(length_penalty) * math.log2(max_tokens) > 1000:
+        raise ValueError(f"a length penalty of {length_penalty} takes {max_tokens} tokens out of the range of numbers")
     for i, p in enumerate(prompts):
         if len(p) == 0:
             raise ValueError(f"request {i}: the prompt is empty")
