@@ -216,6 +216,27 @@ def test_select_peaked_rows_and_near_ties():
     _check_select(x, scores, 16)
 
 
+@pytest.mark.parametrize("V", [4099, 131072, 262144])
+@pytest.mark.parametrize("n", [1, 16])
+@pytest.mark.parametrize("top", [0.0, 7.3, -250.7])
+def test_select_rows_whose_weight_lies_below_the_bound(V, n, top):
+    """`n` entries, and all others one height below them, so that nearly all exps run in 32 bits and are rounded alike: a row's logarithm is off
+    by less than 2^-19 (beam_select.cu).  Scores near it, so that values are near zero and their own rounding hides nothing."""
+    from torchless_rs_b200.sampling import BeamSelector
+    dev = torch.device("cuda")
+    for part in range(4):
+        low = (np.float32(top) - np.linspace(0.02 + 3.4 * part, 3.4 * part + 3.4, 64)).astype(np.float32)
+        high = np.float32(top)
+        x = np.repeat(low[:, None], V, axis=1)
+        x[:, 5:5 + 3 * n:3] = high
+        lse = np.float64(high) + np.log(n + (V - n) * np.exp(low.astype(np.float64) - np.float64(high)))
+        scores = (lse - np.float64(high)).astype(np.float32)[:, None]
+        v, _, t = BeamSelector(dev).select(torch.from_numpy(x).to(dev), torch.from_numpy(scores).to(dev), n)
+        want = scores[:, 0].astype(np.float64) + (np.float64(high) - lse)
+        assert (t.cpu().numpy() == 5 + 3 * np.arange(n)).all()
+        assert (np.abs(v.cpu().numpy().astype(np.float64) - want[:, None]) <= 2.0 ** -19 + np.abs(want[:, None]) * 2.0 ** -24).all()
+
+
 def test_select_strided_and_misaligned_rows():
     rng = np.random.default_rng(9)
     whole = torch.from_numpy(rng.standard_normal((12, 5003)).astype(np.float32)).cuda()

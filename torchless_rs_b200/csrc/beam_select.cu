@@ -13,9 +13,12 @@
 // in 64 bits and ranked by counting.  The second kernel, a block per sequence, joins the parts of each row and takes the n
 // largest of their candidates the same way.
 //
-// Candidates of different beams are compared by sums of 32-bit numbers whose logarithm is rounded too, so which comes first is decided
-// in 64 bits: the entries with weight are those that are collected; the exp of the others runs in 32 bits, and their results are added
-// without rounding (below).
+// Candidates are compared by sums in 64 bits, and the logarithm is taken in 64.  What goes into it is less exact: the collected entries' exp
+// runs in 64 bits, that of the others in 32, and their results are added without rounding (below).  An entry d = bound - x below the bound
+// has an exponent d log2 e, rounded (with the difference and the constant) by less than 1.5 x 2^-20 for d up to 11, and ex2 and a change of the
+// bound add 2^-22 each; entries further below have no weight beside the bound's n unless there are more than 2^17 of them.  So a row's
+// logarithm is off by less than 2^-19 where it has up to 2^18 entries (2^-20.9 was the most that rows made for it gave), the same for all
+// candidates of a beam: their order is that of the logits, and candidates of different beams that are closer than 2^-18 may change places.
 //
 // What bounds it: for many rows the reading of the logits, for few the chain of small steps (loads, barriers, 64-bit exp and log).
 // Measured: 64 sequences x 8 beams x 131072 entries, 268 MB: 58 us (4.6 TB/s); 8 x 4 x 32000: 9 us; 1 x 2 x 256: 7 us, 4 of them the
