@@ -23,10 +23,12 @@ MAX_PARTS = 160                # pieces of a unit that the merge takes
 # differ, one block for all beams' own pages), which read what rows share from the L2 cache at up to 9 TB/s; so the bytes of keys and values
 # that rows need not read again have to exceed `bytes` and `share` of those that rows hold alone.  Measured over 1296 shapes (1 to 16
 # groups of 2 to 8 rows, 64 to 4096 common and 20 to 1000 own tokens, six head layouts, cold cache), per row / shared: bfloat16, 32 over
-# 8 heads of 128, 4 groups of 4: 256 + 200 tokens 10.0 / 14.2 us, 1024 + 20 14.4 / 14.2, 4096 + 20 38 / 20; 16 groups of 8 with 4096 +
-# 20 239 / 63; 32-bit, 1 group of 8, 256 + 20 14.1 / 14.8, 1024 + 20 31 / 21.  The rule is 0.5 % (bfloat16) and 3 % (32-bit) above the better of
-# both in the geometric mean; always per row 12 % and 49 %, always shared 37 % and 5 %.
-WORTH = {torch.bfloat16: (50e6, 0.5), torch.float32: (5e6, 0.0)}
+# 8 heads of 128, 4 groups of 4: 256 + 200 tokens 9.9 / 14.0 us, 1024 + 20 14.4 / 14.1, 4096 + 20 38 / 20; 16 groups of 8 with 4096 +
+# 20 239 / 63; 32-bit, 1 group of 8, 256 + 20 14.1 / 14.9, 1024 + 20 31 / 21; 4 groups of 4, 64 + 20 8.7 / 14.5.  The rule is 0.4 % (bfloat16)
+# and 3 % (32-bit) above the better of both in the geometric mean; always per row 12 % and 49 %, always shared 37 % and 5 %.  At its worst it
+# takes 25 % longer than the other kernel would (bfloat16, 32 over 4 heads of 64, 16 groups of 8, 1024 + 1000: 39.6 / 49.5; more than 10 % on
+# 10 of 648 shapes) and 84 % (32-bit, the same heads, 16 groups of 2, 64 + 1000: 54.4 / 29.6, where the per-row kernel is slow; 69 of 648).
+WORTH = {torch.bfloat16: (50e6, 0.5), torch.float32: (7.5e6, 0.0)}
 
 for _hd in HEAD_DIMS:
     build.register_library(f"attn_shared_bf16_hd{_hd}", ("attention_shared.cu",), (f"-DHEAD_DIM={_hd}",))
