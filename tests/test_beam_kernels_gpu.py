@@ -237,6 +237,37 @@ def test_select_rows_whose_weight_lies_below_the_bound(V, n, top):
         assert (np.abs(v.cpu().numpy().astype(np.float64) - want[:, None]) <= 2.0 ** -19 + np.abs(want[:, None]) * 2.0 ** -24).all()
 
 
+@pytest.mark.parametrize("V,n", [(50, 12), (5000, 16), (20001, 33), (70000, 8), (70000, 100)])
+@pytest.mark.parametrize("rows", [2, 600])
+@pytest.mark.parametrize("case", ["scores", "infinite", "tiny"])
+def test_select_sums_that_are_equal_though_logits_are_not(V, n, rows, case):
+    """Sums so far from zero (or logits so near it) that different logits of a beam have the same sum in 64 bits: the larger logit comes
+    first, of equal ones the lower token, whatever the number of rows (which says how a row is cut)."""
+    from torchless_rs_b200.sampling import BeamSelector
+    dev = torch.device("cuda")
+    rng = np.random.default_rng(V + n)
+    x = rng.standard_normal((2, V)).astype(np.float32)
+    scores = np.array([[-30.0, -31.0]], dtype=np.float32)
+    if case == "scores":
+        x[:, ::3] = np.round(x[:, ::3])
+        scores = np.array([[-1e30, -1e30]], dtype=np.float32)
+    elif case == "infinite":
+        x[0, rng.permutation(V)[:n // 2]] = np.inf
+        x[1] = -np.inf
+    else:
+        x = (x * np.float32(1e-25)).astype(np.float32)
+    order = np.argsort(-x, axis=1, kind="stable")[:, :n]
+    top = [np.nan_to_num(x[b].astype(np.float64), posinf=F32_MAX, neginf=-np.inf) for b in range(2)]
+    sums = [float(scores[0, b]) + (t - (t.max() + np.log(np.exp(t - t.max()).sum()) if t.max() > -np.inf else 0.0)) for b, t in enumerate(top)]
+    found = sorted([(-sums[b][t], b, -top[b][t], int(t)) for b in range(2) for t in order[b] if sums[b][t] > -np.inf])[:n]
+    S = rows // 2
+    lt = torch.from_numpy(np.tile(x, (S, 1))).to(dev)
+    _, b, t = BeamSelector(dev).select(lt, torch.from_numpy(np.tile(scores, (S, 1))).to(dev), n)
+    want_b, want_t = torch.tensor([f[1] for f in found]), torch.tensor([f[3] for f in found])
+    assert len(found) == n
+    assert (b.cpu() == want_b).all() and (t.cpu() == want_t).all()
+
+
 def test_select_strided_and_misaligned_rows():
     rng = np.random.default_rng(9)
     whole = torch.from_numpy(rng.standard_normal((12, 5003)).astype(np.float32)).cuda()

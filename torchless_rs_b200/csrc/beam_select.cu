@@ -377,17 +377,33 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, int V, const fl
   }
 }
 
-// A candidate's value as a word that orders as it does; 0: none.  Both zeros are one.
+// A candidate's value as a word that orders as it does (0: none; both zeros are one), and what comes first where values are equal: the lower
+// beam (10 bits), its larger logit (32 bits; sums far from zero may be equal where logits are not), the lower token (22 bits: the place in the beam's lists of
+// candidates, which have equal logits in the order of their tokens).
 struct __align__(16) BsCand {
   u64 v;
-  uint32_t at;          // beam * V + token
+  u64 tie;
 };
+#define BS_NONE ~0ull
+#define BS_PLACE_BITS 22
+#define BS_BEAM_SHIFT (32 + BS_PLACE_BITS)
 __device__ __forceinline__ u64 bs_key64(double x) {
   const u64 u = (u64)__double_as_longlong(x + 0.0);
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 __device__ __forceinline__ double bs_value64(u64 k) { return __longlong_as_double((long long)(k >> 63 ? k & 0x7fffffffffffffffull : ~k)); }
-__device__ __forceinline__ bool bs_before(const BsCand& a, const BsCand& b) { return (a.v > b.v) | ((a.v == b.v) & (a.at < b.at)); }
+// 1 where a comes before b: the borrow of (b.v, a.tie) - (a.v, b.tie) as numbers of 128 bits.  (As an expression it becomes a branch where the
+// first half ties: 64 x 8 x 50257 entries 39.2 us.)
+__device__ __forceinline__ int bs_before(const BsCand& a, const BsCand& b) {
+  int borrow;
+  asm("{\n\t.reg .u64 t;\n\t"
+      "sub.cc.u64 t, %1, %2;\n\t"
+      "subc.cc.u64 t, %3, %4;\n\t"
+      "subc.u32 %0, 0, 0;\n\t}"
+      : "=r"(borrow)
+      : "l"(a.tie), "l"(b.tie), "l"(b.v), "l"(a.v));
+  return -borrow;
+}
 // How many of list[0 .. c) come before `mine`.  (Eight loads, then comparisons without branches: taken one by one, with the second half of a
 // comparison only where the first ties, 32 of them took 7000 cycles and the whole selection half as long again.)
 __device__ __forceinline__ int bs_rank(const BsCand* list, int c, const BsCand& mine) {
@@ -397,50 +413,52 @@ __device__ __forceinline__ int bs_rank(const BsCand* list, int c, const BsCand& 
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = list[k + i];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) rank += bs_before(o[i], mine) ? 1 : 0;
+    for (int i = 0; i < 8; ++i) rank += bs_before(o[i], mine);
   }
 #pragma unroll 1
-  for (; k < c; ++k) rank += bs_before(list[k], mine) ? 1 : 0;
+  for (; k < c; ++k) rank += bs_before(list[k], mine);
   return rank;
 }
 __device__ __forceinline__ BsCand bs_shfl(const BsCand& a, int o) {
-  return {__shfl_xor_sync(0xffffffffu, a.v, o), __shfl_xor_sync(0xffffffffu, a.at, o)};
+  return {__shfl_xor_sync(0xffffffffu, a.v, o), __shfl_xor_sync(0xffffffffu, a.tie, o)};
 }
 
 // CAND: candidates of a sequence per thread that are held in registers; 0: any number, read again for every look at them.  (The bound on
 // registers is for the order of the code: without it 64 sequences of 8 beams take 4 us more.)
 template <int GS, int CAND>
 __global__ void __launch_bounds__(BS_THREADS, 4)
-beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ cand, const float* __restrict__ scores, int B, int V,
+beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ cand, const float* __restrict__ scores, int B,
                   int n, int parts, float* __restrict__ values, int* __restrict__ beams, int* __restrict__ tokens) {
   constexpr int GROUPS = BS_THREADS / GS, HELD = CAND ? CAND : 1;
   extern __shared__ double lse[];         // [B]
   __shared__ BsCand gm[GROUPS];
   __shared__ BsCand buf[BS_CAP];
+  __shared__ uint32_t token_of[BS_CAP];
   __shared__ BsCand bound;
   __shared__ int count;
   const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t row0 = (size_t)s * B;
   const int total = B * parts * n;
-  const BsCand none = {0, 0xffffffffu};
+  const BsCand none = {0, BS_NONE};
   if (tid == 0) count = 0;
   pdl_wait();
   pdl_launch_dependents();
   // candidate i: its value without its beam's share, and which beam's; everything is on its way before the first is waited for
   struct Raw {
-    float x, score;
+    uint32_t key, token;
+    float score;
     int beam, left;                       // left: how many follow it and itself; none if it is not positive
-    uint32_t token;
   };
   auto raw = [&](int i) -> Raw {
-    if (i >= total) return {0.0f, 0.0f, 0, 0, 0u};
+    if (i >= total) return {0u, 0u, 0.0f, 0, 0};
     const int k = i / n, b = k / parts;
     const uint2 c = cand[row0 * parts * n + i];
-    return {bs_value(c.x), scores[row0 + b], b, part[row0 * parts + k].count - (i - k * n), c.y};
+    return {c.x, c.y, scores[row0 + b], b, part[row0 * parts + k].count - (i - k * n)};
   };
-  auto value = [&](const Raw& r) -> BsCand {
+  auto value = [&](const Raw& r, int i) -> BsCand {
     if (r.left <= 0) return none;
-    return {bs_key64((double)r.score + ((double)r.x - lse[r.beam])), (uint32_t)r.beam * (uint32_t)V + r.token};
+    return {bs_key64((double)r.score + ((double)bs_value(r.key) - lse[r.beam])),
+            (u64)r.beam << BS_BEAM_SHIFT | (u64)~r.key << BS_PLACE_BITS | (uint32_t)(i - r.beam * parts * n)};
   };
   auto part_of = [&](int b) -> BsPart {
     if (b < B && lane < parts) return part[(row0 + b) * parts + lane];
@@ -476,12 +494,12 @@ beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ can
   if (CAND) {
 #pragma unroll
     for (int j = 0; j < HELD; ++j) {
-      mine[j] = value(held[j]);
+      mine[j] = value(held[j], tid + j * BS_THREADS);
       if (bs_before(mine[j], best)) best = mine[j];
     }
   } else {
     for (int i = tid; i < total; i += BS_THREADS) {
-      const BsCand e = value(raw(i));
+      const BsCand e = value(raw(i), i);
       if (bs_before(e, best)) best = e;
     }
   }
@@ -490,7 +508,7 @@ beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ can
     const BsCand other = bs_shfl(best, o);
     if (bs_before(other, best)) best = other;
   }
-  if (best.v == 0) best.at = 0xffffffffu - tid / GS;       // (empty groups come one after the other)
+  if (best.v == 0) best.tie = BS_NONE - tid / GS;          // (empty groups come one after the other)
   if (tid % GS == 0) gm[tid / GS] = best;
   __syncthreads();
   if (tid < GROUPS) {
@@ -500,19 +518,25 @@ beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ can
   }
   __syncthreads();
   BsCand bd = bound;
-  auto collect = [&](const BsCand& e) {
-    if (e.at != 0xffffffffu && !bs_before(bd, e)) {
+  auto collect = [&](const BsCand& e, uint32_t token) {
+    if (e.tie != BS_NONE && !bs_before(bd, e)) {
       const int at = atomicAdd(&count, 1);
-      if (at < BS_CAP) buf[at] = e;
+      if (at < BS_CAP) {
+        buf[at] = e;
+        token_of[at] = token;
+      }
     }
   };
   if (CAND) {                             // (held candidates are at most as many as there is room for)
 #pragma unroll
-    for (int j = 0; j < HELD; ++j) collect(mine[j]);
+    for (int j = 0; j < HELD; ++j) collect(mine[j], held[j].token);
     __syncthreads();
   } else {
     for (;;) {
-      for (int i = tid; i < total; i += BS_THREADS) collect(value(raw(i)));
+      for (int i = tid; i < total; i += BS_THREADS) {
+        const Raw r = raw(i);
+        collect(value(r, i), r.token);
+      }
       __syncthreads();
       if (count <= BS_CAP) break;
       // more reach the bound than there is room for: the n-th of those collected is the next one (which leaves out all but n of them)
@@ -528,22 +552,22 @@ beam_merge_kernel(const BsPart* __restrict__ part, const uint2* __restrict__ can
   }
   const int c = count;
   const size_t o0 = (size_t)s * n;
-  auto put = [&](int r, const BsCand& e) {
+  auto put = [&](int r, const BsCand& e, int token) {
     const double v = bs_value64(e.v);
-    const bool got = e.at != 0xffffffffu && v > -INFINITY;
-    const uint32_t beam = e.at / (uint32_t)V;
+    const bool got = e.tie != BS_NONE && v > -INFINITY;
     values[o0 + r] = got ? (float)v : -INFINITY;
-    beams[o0 + r] = got ? (int)beam : -1;
-    tokens[o0 + r] = got ? (int)(e.at - beam * (uint32_t)V) : -1;
+    beams[o0 + r] = got ? (int)(e.tie >> BS_BEAM_SHIFT) : -1;
+    tokens[o0 + r] = got ? token : -1;
   };
   for (int i = tid; i < max(c, n); i += BS_THREADS) {
     BsCand e = none;
-    int rank = i;                         // places without a candidate
+    int rank = i, token = -1;             // places without a candidate
     if (i < c) {
       e = buf[i];
+      token = (int)token_of[i];
       rank = bs_rank(buf, c, e);
     }
-    if (rank < n) put(rank, e);
+    if (rank < n) put(rank, e, token);
   }
 }
 
@@ -572,6 +596,7 @@ static int bs_run(const float* logits, long long ld, int S, int B, int V, const 
   // tiles gain no more.)
   while ((long long)B * bs_parts(V, chunk, shifted) * n > 4 * BS_THREADS && chunk < 8 * BS_TILE && chunk < V) chunk *= 2;
   const int parts = bs_parts(V, chunk, shifted);
+  if ((long long)parts * n >= 1ll << BS_PLACE_BITS) return -2;     // (2^30 entries have some 2^13 parts)
   BsPart* part = (BsPart*)scratch;
   uint2* cand = (uint2*)(part + (size_t)rows * parts);
   const int st = alike ? tl_launch(beam_rows_kernel<GS, true>, dim3(parts, rows), dim3(BS_THREADS), 0, stream, logits, ld, V, scores, n, chunk, part, cand)
@@ -580,7 +605,7 @@ static int bs_run(const float* logits, long long ld, int S, int B, int V, const 
   const long long total = (long long)B * parts * n;
   auto merge = [&](auto kernel) {
     return tl_launch(kernel, dim3(S), dim3(BS_THREADS), (size_t)B * sizeof(double), stream, (const BsPart*)part, (const uint2*)cand, scores, B,
-                     V, n, parts, values, beams, tokens);
+                     n, parts, values, beams, tokens);
   };
   return total <= BS_THREADS ? merge(beam_merge_kernel<GS, 1>) : total <= 4 * BS_THREADS ? merge(beam_merge_kernel<GS, 4>) : merge(beam_merge_kernel<GS, 0>);
 }
@@ -592,7 +617,7 @@ extern "C" int tl_beam_select(const float* logits, long long ld, int S, int B, i
   if (S <= 0) return 0;
   if (B <= 0 || V <= 0 || n <= 0 || ld < V || ((uintptr_t)logits & 3)) return -1;
   if (V > (1 << 30)) return -2;
-  if (n > BS_MAX_N || B > 1024 || (long long)S * B > 65535 || (long long)B * V >= 0x7fffffffLL ||
+  if (n > BS_MAX_N || B > 1 << (64 - BS_BEAM_SHIFT) || (long long)S * B > 65535 || (long long)B * V >= 0x7fffffffLL ||
       (long long)B * bs_parts(V, BS_TILE, true) * n >= 0x7fffffffLL)
     return -2;
   // twice as many groups as entries are asked for, where there are
